@@ -85,9 +85,11 @@ def _flags(kind: str, incs, abi):
     common = ["-O3", "-fPIC", "-std=c++17", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-I{CSRC}",
               "-Wno-unused-result", "-Wno-deprecated-declarations"]
     if kind == "hip":
-        # Device code: gfx950 only. -ffp-contract=fast lets hipcc fuse mul+add into v_fma/v_pk_fma.
-        return common + [f"--offload-arch={ARCH}", "-ffp-contract=fast", "-munsafe-fp-atomics",
-                         "-fgpu-rdc" if False else "-fno-gpu-rdc"]
+        # Device code: gfx950 only. -ffp-contract=fast lets hipcc fuse mul+add into v_fma.  Packed fp32
+        # (v_pk_add / mul / fma_f32) is off: some of its forms have given wrong results now and then,
+        # without an error; the scalar forms round the same.
+        return common + [f"--offload-arch={ARCH}", "-ffp-contract=fast", "-munsafe-fp-atomics", "-fno-gpu-rdc",
+                         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     py_inc = sysconfig.get_paths()["include"]
     torch_flags = [f"-I{i}" for i in incs] + [f"-I{py_inc}", f"-I{ROCM}/include",
                                              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",

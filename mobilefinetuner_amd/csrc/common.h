@@ -123,10 +123,9 @@ __device__ __forceinline__ void gelu_tanh_and_grad(float x, float& y, float& dy)
   dy = s + 2.f * x * s * (1.f - s) * k0 * (1.f + 3.f * k1 * x2);
 }
 
-// Two elements at once in packed fp32 (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32 on gfx950: two lanes'
-// worth per instruction), the constants folded: 10 packed ops + 2 v_exp_f32 + 2 v_rcp_f32 per pair
-// instead of ~14 scalar ops + 2 transcendentals per element -- the GELU epilogue of the fused MLP GEMM
-// was VALU-bound at one wave per SIMD (as many cycles as the tile's MFMAs).
+// Two elements at once as float2 arithmetic with the constants folded: ~10 mul / fma per element and 2
+// v_exp_f32 + 2 v_rcp_f32 per pair.  (Compiled to scalar fp32 instructions: the build turns packed fp32
+// off, which costs the headline step 0.6 % and is bit-identical.)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_tanh_and_grad2(f32x2_t x, f32x2_t& y, f32x2_t& dy) {
   const float k0 = 0.7978845608028654f, k1 = 0.044715f, l2e = 1.4426950408889634f;

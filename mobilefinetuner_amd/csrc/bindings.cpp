@@ -316,6 +316,114 @@ Tensor logsoftmax_gather(Tensor logits, Tensor idx, int64_t V) {
   return out;
 }
 
+// ------------------------------------------------------------------ 4-bit frozen weights
+// codes [N, K / 2], scales [N, K / 32] (ops/mx4.py MX4Weight); returns {N, K}
+std::pair<long, int> mx4_shape(const Tensor& codes, const Tensor& scales, const char* what) {
+  TORCH_CHECK(codes.is_cuda() && scales.is_cuda() && codes.device() == scales.device(), what,
+              ": codes and scales must be on one GPU");
+  TORCH_CHECK(codes.scalar_type() == torch::kUInt8 && scales.scalar_type() == torch::kUInt8 && codes.dim() == 2 &&
+                  scales.dim() == 2 && codes.is_contiguous() && scales.is_contiguous(),
+              what, ": codes and scales must be contiguous 2-D uint8 tensors");
+  const long N = codes.size(0), K = codes.size(1) * 2;
+  TORCH_CHECK(K > 0 && K % 32 == 0 && K <= 0x3fffffff && N <= 0x3fffffff && scales.size(0) == N && scales.size(1) == K / 32, what,
+              ": codes [N, K / 2] with K % 32 == 0 and scales [N, K / 32]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, what, ": codes must start at a 16-byte boundary");
+  return {N, (int)K};
+}
+const uint8_t* u8p(const Tensor& t) { return t.data_ptr<uint8_t>(); }
+bool rows16(const Tensor& t) {  // 2-D bf16 rows that 16-byte loads may walk
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+std::vector<Tensor> mx4_quantize(Tensor w) {
+  CHECK_CUDA(w);
+  const bool f32 = w.scalar_type() == torch::kFloat32;
+  TORCH_CHECK(f32 || w.scalar_type() == torch::kBFloat16, "mx4_quantize: W must be fp32 or bf16");
+  TORCH_CHECK(w.dim() == 2 && w.size(1) > 0 && w.size(1) % 32 == 0, "mx4_quantize: W [N, K] with K a multiple of 32");
+  TORCH_CHECK(w.size(0) <= 0x3fffffff && w.size(1) <= 0x3fffffff, "mx4_quantize: W has too many rows or columns");
+  c10::DeviceGuard g(w.device());
+  w = w.contiguous();
+  if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) w = w.clone();
+  const long N = w.size(0), K = w.size(1);
+  auto codes = torch::empty({N, K / 2}, w.options().dtype(torch::kUInt8));
+  auto scales = torch::empty({N, K / 32}, w.options().dtype(torch::kUInt8));
+  mft::mx4_quantize(w.data_ptr(), f32, codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), N, (int)K, stream());
+  return {codes, scales};
+}
+
+Tensor mx4_dequantize(Tensor codes, Tensor scales) {
+  const auto [N, K] = mx4_shape(codes, scales, "mx4_dequantize");
+  c10::DeviceGuard g(codes.device());
+  auto out = torch::empty({N, K}, codes.options().dtype(torch::kBFloat16));
+  mft::mx4_dequantize(u8p(codes), u8p(scales), 0, N, K, bp(out), K, N, K, stream());
+  return out;
+}
+
+Tensor mx4_embed(Tensor ids, Tensor codes, Tensor scales, c10::optional<Tensor> wpe, double scale) {
+  const auto [N, K] = mx4_shape(codes, scales, "mx4_embedding");
+  TORCH_CHECK(ids.is_cuda() && ids.device() == codes.device() && ids.scalar_type() == torch::kInt64 && ids.dim() == 2,
+              "mx4_embedding: ids [B, S] must be int64 on the table's GPU");
+  TORCH_CHECK(N > 0, "mx4_embedding: the table has no rows");
+  const long S = ids.size(1), M = ids.numel();
+  if (wpe.has_value()) {
+    TORCH_CHECK(wpe->is_cuda() && wpe->device() == codes.device() && wpe->scalar_type() == torch::kBFloat16 && wpe->dim() == 2 &&
+                    wpe->is_contiguous() && wpe->size(1) == K && wpe->size(0) >= S &&
+                    reinterpret_cast<uintptr_t>(wpe->data_ptr()) % 16 == 0,
+                "mx4_embedding: wpe must be contiguous bf16 [>= S, C] on the table's GPU");
+  }
+  c10::DeviceGuard g(codes.device());
+  ids = ids.contiguous();
+  auto out = torch::empty({M, K}, codes.options().dtype(torch::kBFloat16));
+  mft::mx4_embed(ids.data_ptr<int64_t>(), u8p(codes), u8p(scales), N, K, optp<bf16_t>(wpe), bp(out), M, (int)S, (float)scale,
+                 stream());
+  return out;
+}
+
+// the [rows, width] operand of an mx4 product: itself where 16-byte loads may walk it, else a copy; `zpad`:
+// columns past the width up to the next multiple of 8 are read and have to be zeros
+Tensor mx4_operand(const Tensor& x, long width, bool zpad) {
+  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, width});
+  if (rows16(x2) && !(zpad && width % 8)) return x2;
+  auto c = (zpad && width % 8) ? torch::zeros({x2.size(0), (width + 7) / 8 * 8}, x2.options())
+                               : torch::empty({x2.size(0), (width + 7) / 8 * 8}, x2.options());
+  c.narrow(1, 0, width).copy_(x2);
+  return c;
+}
+
+Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, const c10::optional<Tensor>& bias, bool dgrad) {
+  const char* what = dgrad ? "mx4_linear's gradient" : "mx4_linear";
+  const auto [N, K] = mx4_shape(codes, scales, what);
+  TORCH_CHECK(x.is_cuda() && x.device() == codes.device(), what, ": the activation must be on the weight's GPU");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16, what, ": the activation must be bf16");
+  const long in = dgrad ? N : K, out = dgrad ? K : N;
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == in, what, ": expected [.., ", in, "], got ", x.sizes());
+  if (bias.has_value() && bias->defined())
+    TORCH_CHECK(bias->is_cuda() && bias->device() == codes.device() && bias->scalar_type() == torch::kBFloat16 &&
+                    bias->is_contiguous() && bias->numel() == N,
+                what, ": the bias must be contiguous bf16 [", N, "] on the weight's GPU");
+  c10::DeviceGuard g(codes.device());
+  auto sizes = x.sizes().vec();
+  sizes.back() = out;
+  auto y = torch::empty(sizes, x.options());
+  if (y.numel() == 0) return y;
+  if (in == 0) return y.zero_();
+  const Tensor x2 = mx4_operand(x, in, dgrad);
+  TORCH_CHECK(x2.size(0) <= 0x3fffffff, what, ": too many rows");
+  mft::Mx4LinearArgs a{};
+  a.codes = u8p(codes); a.scales = u8p(scales);
+  a.x = bp(x2); a.ldx = x2.stride(0);
+  a.bias = optp<bf16_t>(bias);
+  a.y = bp(y); a.ldy = out;
+  a.M = (int)x2.size(0); a.N = (int)N; a.K = K;
+  if (dgrad) mft::mx4_dgrad(a, stream());
+  else mft::mx4_linear(a, stream());
+  return y;
+}
+Tensor mx4_linear(Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> bias) {
+  return mx4_product(x, codes, scales, bias, false);
+}
+Tensor mx4_dgrad(Tensor dy, Tensor codes, Tensor scales) { return mx4_product(dy, codes, scales, c10::nullopt, true); }
+
 // ------------------------------------------------------------------ optimizer
 void sumsq(Tensor x, Tensor out, bool accumulate) {
   CHECK_F32(x); CHECK_CONTIG(x);
@@ -734,6 +842,11 @@ PYBIND11_MODULE(_C, m) {
   m.def("ce_dgrad_splits", &mft::ce_dgrad_splits, "vocab splits of the LM-head CE dgrad for an M-row chunk");
   m.def("lora_dy_grid_blocks", &mft::lora_dy_grid_blocks, "workgroups of the lora_dy / lora_xty grids");
   m.def("logsoftmax_gather", &logsoftmax_gather);
+  m.def("mx4_quantize", &mx4_quantize);
+  m.def("mx4_dequantize", &mx4_dequantize);
+  m.def("mx4_embed", &mx4_embed);
+  m.def("mx4_linear", &mx4_linear);
+  m.def("mx4_dgrad", &mx4_dgrad);
   m.def("sumsq", &sumsq);
   m.def("nonfinite_check", &nonfinite_check);
   m.def("adamw_step", &adamw_step, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("lr"),

@@ -358,6 +358,30 @@ void qknorm_rope_bwd(const bf16_t* x, const long* st, const bf16_t* dy, const fl
                      const long* dst, float* dw, float* work, int B, int S, int H, int D, const float* cos_t,
                      const float* sin_t, int pos0, float off, int interleaved, int accumulate, hipStream_t stream);
 
+// ---------------------------------------------------------------- 4-bit frozen weights (mx4.hip)
+// W [N, K], K % 32 == 0: e2m1 codes [N, K / 2] (even column in the low half-byte) and scale bytes [N, K / 32],
+// value = e2m1(code) * 2^(byte - 127), byte 255 = NaN.  Every value is exact in bf16.  Codes 16-B aligned.
+// w: contiguous, 16-B aligned, fp32 or bf16
+void mx4_quantize(const void* w, int w_f32, uint8_t* codes, uint8_t* scales, long N, int K, hipStream_t st);
+// out[r, :] = W[n0 + r] for r < rows (rows past N: zeros), columns K .. kpad - 1 zeros (kpad, ldo % 8 == 0)
+void mx4_dequantize(const uint8_t* codes, const uint8_t* scales, long n0, long N, int K, bf16_t* out, long ldo, long rows,
+                    int kpad, hipStream_t st);
+// out[m] = W[ids[m]] * scale (+ wpe[m % S]); a row of NaN for an id outside [0, N)
+void mx4_embed(const int64_t* ids, const uint8_t* codes, const uint8_t* scales, long N, int K, const bf16_t* wpe,
+               bf16_t* out, long M, int S, float scale, hipStream_t st);
+struct Mx4LinearArgs {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const bf16_t* x;  // linear: x [M, K]; dgrad: dy [M, N] (N % 8 == 0, or its columns N .. up to 8 are zeros)
+  long ldx;         // % 8 == 0, 16-B aligned rows
+  const bf16_t* bias;  // linear: [N] or null
+  bf16_t* y;        // linear: y [M, N]; dgrad: dx [M, K] (ldy % 4 == 0, 8-B aligned)
+  long ldy;
+  int M, N, K;
+};
+void mx4_linear(const Mx4LinearArgs& a, hipStream_t st);  // y = x W^T + bias
+void mx4_dgrad(const Mx4LinearArgs& a, hipStream_t st);   // dx = dy W
+
 // ---------------------------------------------------------------- misc (misc.hip)
 void cast_f32_bf16(const float* x, bf16_t* y, long n, hipStream_t st);
 void cast_bf16_f32(const bf16_t* x, float* y, long n, hipStream_t st);

@@ -24,6 +24,7 @@ import torch
 from torch.autograd import Function
 
 from .._ext import native
+from .mx4 import MX4Weight
 
 GEMM_EPI_NONE, GEMM_EPI_BIAS, GEMM_EPI_BIAS_GELU, GEMM_EPI_DGELU, GEMM_EPI_F32ACC, GEMM_EPI_LORA = 0, 1, 2, 3, 4, 5
 GEMM_EPI_BIAS_GELU_D, GEMM_EPI_MUL_AUX = 9, 10
@@ -301,7 +302,9 @@ class _Embedding(Function):
 
 @_device_op
 def embedding(ids, wte, wpe=None, scale=1.0):
-    """ids [B,S] -> [B*S, C]: wte[ids]*scale (+ wpe[pos])."""
+    """ids [B,S] -> [B*S, C]: wte[ids]*scale (+ wpe[pos]); wte may be an MX4Weight."""
+    if isinstance(wte, MX4Weight):
+        return mx4_embedding(ids, wte, wpe, scale)
     B, S = ids.shape
     return _Embedding.apply(ids, wte, wpe, S, float(scale))
 
@@ -517,6 +520,8 @@ def _g8_ok(x2, *ts) -> bool:
 
 def gemm_linear(x2, wc, bc=None):
     """y = x W^T (+ b), W [out, in]."""
+    if isinstance(wc, MX4Weight):
+        return native().mx4_linear(x2, wc.codes, wc.scales, bc)
     M, K = x2.shape
     N = wc.shape[0]
     if _gemm8_all() and _g8_ok(x2, wc) and K % 64 == 0 and N % 8 == 0 and (bc is None or bc.dtype == torch.bfloat16):
@@ -528,6 +533,8 @@ def gemm_linear(x2, wc, bc=None):
 
 def gemm_dx(dy2, wc, out=None):
     """dx = dy W (W [out, in], possibly a row-strided view) -- gemm8 NN."""
+    if isinstance(wc, MX4Weight):
+        return native().mx4_dgrad(dy2, wc.codes, wc.scales)
     N = wc.shape[0]
     if _g8_ok(dy2, wc) and N % 64 == 0 and wc.shape[1] % 8 == 0 and (out is None or _g8_ok(out)):
         return native().gemm_t(dy2, wc, False, True, GEMM_EPI_NONE, out=out)[0]
@@ -600,8 +607,56 @@ class _Linear(Function):
 
 @_device_op
 def linear(x, w, b=None):
-    """y = x W^T + b with W [out, in] (nn.Linear layout)."""
+    """y = x W^T + b with W [out, in] (nn.Linear layout); W may be an MX4Weight."""
+    if isinstance(w, MX4Weight):
+        return mx4_linear(x, w, b)
     return _Linear.apply(x, w, b)
+
+
+# ---------------------------------------------------------------- 4-bit frozen weights
+@_device_op
+def mx4_quantize(w) -> MX4Weight:
+    """W [N, K] (fp32 or bf16, K a multiple of 32) in 4 bits.  Per 32 columns of a row the scale is the power
+    of two under which the largest magnitude lies in (3.5, 7] (over 6 it saturates, off by at most half a
+    step), then nearest code, ties to even.  A group that holds an infinity or a NaN reads as NaN."""
+    return MX4Weight(*native().mx4_quantize(w.detach()))
+
+
+@_device_op
+def mx4_dequantize(codes, scales):
+    """The values of an MX4Weight's two tensors, bf16 [N, K] (every one exact)."""
+    return native().mx4_dequantize(codes, scales)
+
+
+class _MX4Linear(Function):
+    @staticmethod
+    def forward(ctx, x, w, b):
+        ctx.w, ctx.b = w, b
+        return native().mx4_linear(x, w.codes, w.scales, cw(b))
+
+    @staticmethod
+    def backward(ctx, dy):
+        w, b = ctx.w, ctx.b
+        dx = native().mx4_dgrad(dy, w.codes, w.scales) if ctx.needs_input_grad[0] else None
+        return dx, None, (_bias_grad(b, dy.reshape(-1, dy.shape[-1])) if _needs(b) else None)
+
+
+@_device_op
+def mx4_linear(x, w, b=None):
+    """y = x W^T + b for an MX4Weight W [out, in]: x bf16 [.., in] of one row or many -> [.., out].  The
+    gradient goes to x (and to b); W is frozen."""
+    if torch.is_grad_enabled() and (x.requires_grad or _needs(b)):
+        return _MX4Linear.apply(x, w, b)
+    return native().mx4_linear(x, w.codes, w.scales, cw(b))
+
+
+@_device_op
+def mx4_embedding(ids, w, wpe=None, scale=1.0):
+    """ids [B, S] -> bf16 [B*S, C]: W[ids] * scale (+ wpe[position]) for an MX4Weight table, rounded once.  An
+    id outside the table gives a row of NaN.  The table is frozen and the positions are not trained here."""
+    if _needs(wpe):
+        raise RuntimeError("mx4_embedding: the position table is trained by embedding() with a bf16 token table")
+    return native().mx4_embed(ids, w.codes, w.scales, cw(wpe) if wpe is not None else None, float(scale))
 
 
 def frozen_weight_t(p):

@@ -7,9 +7,14 @@ import math
 
 import torch
 
-from mobilefinetuner_amd.ops.functional import rw
+from mobilefinetuner_amd.ops.functional import MX4Weight, rw
 
+from . import mx4
 from . import reference as ref
+
+
+def _w(p):
+    return mx4.values(p.codes, p.scales) if isinstance(p, MX4Weight) else rw(p)
 
 
 def layer_norm(x, w, b, eps=1e-5, out_cols=0):
@@ -40,6 +45,8 @@ def gated_act(gu, act="gelu", out_cols=0):
 
 
 def embedding(ids, wte, wpe=None, scale=1.0):
+    if isinstance(wte, MX4Weight):
+        return mx4_embedding(ids, wte, wpe, scale)
     B, S = ids.shape
     e = rw(wte)[ids.reshape(-1)].float()
     if scale != 1.0:
@@ -77,7 +84,32 @@ def qk_norm_rope_attention(qkv, nq, nkv, wq, wk, cos, sin, eps_q, eps_k, offset=
     return flash_attention(q, k, qkv[:, :, nq + nkv:], scale, True, window, kv_lens)
 
 
+def mx4_quantize(w):
+    return MX4Weight(*mx4.quantize(w.detach()))
+
+
+def mx4_dequantize(codes, scales):
+    return mx4.values(codes, scales).to(torch.bfloat16)
+
+
+def mx4_linear(x, w, b=None):
+    y = x.float() @ mx4.values(w.codes, w.scales).float().t()
+    if b is not None:
+        y = y + rw(b).float()
+    return y.to(x.dtype)
+
+
+def mx4_embedding(ids, w, wpe=None, scale=1.0):
+    B, S = ids.shape
+    e = mx4.values(w.codes, w.scales).float()[ids.reshape(-1)] * scale
+    if wpe is not None:
+        e = e + rw(wpe)[:S].float().repeat(B, 1)
+    return e.to(torch.bfloat16)
+
+
 def linear(x, w, b=None):
+    if isinstance(w, MX4Weight):
+        return mx4_linear(x, w, b)
     y = x.float() @ rw(w).float().t()
     if b is not None:
         y = y + rw(b).float()
@@ -86,7 +118,7 @@ def linear(x, w, b=None):
 
 def lora_linear(x, w, b, slices, scale, training: bool = True):
     xf = x.float()
-    y = xf @ rw(w).float().t()
+    y = xf @ _w(w).float().t()
     if b is not None:
         y = y + rw(b).float()
     parts = []
@@ -105,12 +137,12 @@ def lora_linear(x, w, b, slices, scale, training: bool = True):
 
 
 def lm_head_cross_entropy(h, w, labels, vocab_size, chunk=None, w_grad_scale=1.0):
-    logits = (h.float() @ rw(w).float().t())[:, :vocab_size]
+    logits = (h.float() @ _w(w).float().t())[:, :vocab_size]
     return torch.nn.functional.cross_entropy(logits, labels.reshape(-1), ignore_index=-100)
 
 
 def lm_head_token_nll(h, w, labels, vocab_size, chunk=None):
     with torch.no_grad():
-        logits = (h.float() @ rw(w).float().t())[:, :vocab_size]
+        logits = (h.float() @ _w(w).float().t())[:, :vocab_size]
         nll = torch.nn.functional.cross_entropy(logits, labels.reshape(-1), ignore_index=-100, reduction="sum")
         return nll, (labels >= 0).sum()

@@ -424,6 +424,61 @@ Tensor mx4_linear(Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> b
 }
 Tensor mx4_dgrad(Tensor dy, Tensor codes, Tensor scales) { return mx4_product(dy, codes, scales, c10::nullopt, true); }
 
+// LM-head cross entropy in pieces of the vocabulary (ce_pieces.hip): h [M, K], the table bf16 [>= V, K] or 4-bit
+// [V, K].  Returns {loss (mean over the rows with a label in [0, V)), loss per row, their count, dh or undefined}.
+std::vector<Tensor> lm_head_ce_pieces(Tensor h, c10::optional<Tensor> W, c10::optional<Tensor> codes,
+                                      c10::optional<Tensor> scales, Tensor labels, int64_t V, int64_t piece, bool grad) {
+  const char* what = "lm_head_cross_entropy_pieces";
+  CHECK_CUDA(h); CHECK_BF16(h);
+  TORCH_CHECK(h.dim() == 2, what, ": h must be [M, C]");
+  const long M = h.size(0), K = h.size(1);
+  TORCH_CHECK(labels.is_cuda() && labels.device() == h.device() && labels.scalar_type() == torch::kInt64 && labels.numel() == M,
+              what, ": labels must be int64 [M] on h's GPU");
+  TORCH_CHECK(M <= (1 << 24), what, ": at most 2^24 rows");
+  TORCH_CHECK(piece >= 0 && (piece == 0 || piece % 256 == 0) && piece <= 0x3fffffff, what, ": piece must be a multiple of 256");
+  TORCH_CHECK(V > 0 && V <= 0x3fffffff, what, ": vocab_size must be positive");
+  c10::DeviceGuard g(h.device());
+  const int Kp = (int)((K + 63) / 64 * 64);
+  mft::CePiecesArgs a{};
+  if (W.has_value()) {
+    TORCH_CHECK(W->is_cuda() && W->device() == h.device() && W->scalar_type() == torch::kBFloat16 && W->dim() == 2 &&
+                    W->size(1) == K && W->size(0) >= V, what, ": the table must be bf16 [>= vocab_size, C] on h's GPU");
+    TORCH_CHECK(K > 0 && K % 8 == 0, what, ": C must be a multiple of 8");
+    if (!rows16(*W)) W = W->clone(at::MemoryFormat::Contiguous);
+    a.W = bp(*W); a.ldw = W->stride(0); a.w_rows = W->size(0);
+  } else {
+    TORCH_CHECK(codes.has_value() && scales.has_value(), what, ": a table is needed");
+    const auto [N, Kw] = mx4_shape(*codes, *scales, what);
+    TORCH_CHECK(codes->device() == h.device() && Kw == K && N >= V, what, ": the table must be [>= vocab_size, C] on h's GPU");
+    a.codes = u8p(*codes); a.scales = u8p(*scales);
+  }
+  TORCH_CHECK(K <= 65536, what, ": C must be at most 65536");
+  auto f32 = h.options().dtype(torch::kFloat32);
+  auto loss = torch::empty({}, f32), rows = torch::empty({M}, f32);
+  auto n_valid = torch::empty({}, h.options().dtype(torch::kInt64));
+  Tensor dh;
+  if (grad) dh = torch::empty({M, K}, h.options());
+  if (M == 0) return {loss.zero_(), rows, n_valid.zero_(), dh};
+  labels = labels.contiguous();
+  if (Kp != K) {
+    auto hp = torch::zeros({M, Kp}, h.options());
+    hp.narrow(1, 0, K).copy_(h);
+    h = hp;
+  } else if (!rows16(h)) {
+    h = h.clone(at::MemoryFormat::Contiguous);
+  }
+  a.h = bp(h); a.ldh = h.stride(0);
+  a.labels = labels.data_ptr<int64_t>();
+  a.M = (int)M; a.K = (int)K; a.Kp = Kp; a.V = (int)V;
+  a.piece = piece ? (int)piece : mft::lm_head_ce_pieces_width(M, (int)V);
+  a.loss = fp(loss); a.loss_rows = fp(rows); a.n_valid = n_valid.data_ptr<int64_t>();
+  a.dh = grad ? bp(dh) : nullptr;
+  auto ws = torch::empty({mft::lm_head_ce_pieces_ws_bytes(a)}, h.options().dtype(torch::kUInt8));
+  a.ws = ws.data_ptr();
+  mft::lm_head_ce_pieces(a, stream());
+  return {loss, rows, n_valid, dh};
+}
+
 // ------------------------------------------------------------------ optimizer
 void sumsq(Tensor x, Tensor out, bool accumulate) {
   CHECK_F32(x); CHECK_CONTIG(x);
@@ -847,6 +902,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("mx4_embed", &mx4_embed);
   m.def("mx4_linear", &mx4_linear);
   m.def("mx4_dgrad", &mx4_dgrad);
+  m.def("lm_head_ce_pieces", &lm_head_ce_pieces);
+  m.def("lm_head_ce_pieces_width", &mft::lm_head_ce_pieces_width, "default columns of a vocabulary piece for M rows");
   m.def("sumsq", &sumsq);
   m.def("nonfinite_check", &nonfinite_check);
   m.def("adamw_step", &adamw_step, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("lr"),

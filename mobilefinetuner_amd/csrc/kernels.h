@@ -79,7 +79,9 @@ enum GemmEpi { GEMM_EPI_NONE = 0, GEMM_EPI_BIAS = 1, GEMM_EPI_BIAS_GELU = 2, GEM
                // ldaux), the B rows of each 256-column tile are 128 gate rows + the matching 128 up rows;
                // GEGLU_BWD -- the accumulator is dh [M, I] (N = I); aux = gu [M, 2I] (read), C = dgu
                // [M, 2I] (ldc): dg = dh u gelu'(g), du = dh gelu(g)
-               GEMM_EPI_GEGLU_FWD = 12, GEMM_EPI_GEGLU_BWD = 13 };
+               GEMM_EPI_GEGLU_FWD = 12, GEMM_EPI_GEGLU_BWD = 13,
+               // CE_DGRAD of one piece of the vocabulary, added to a running fp32 sum (gemm8, NN, one split)
+               GEMM_EPI_CE_DGRAD_ACC = 14 };
 struct GemmArgs {
   const bf16_t* A;
   long lda;  // A [M, K] row-major
@@ -137,6 +139,9 @@ struct GemmArgs {
   // gemm_s split-K hand-off: 1 = agent-scope release / acquire fences around the arrival counter
   // (MFT_STRICT_HANDOFF=1); 0 = the sc1-store / sc1-load form alone (see gemm_s.hip)
   int handoff_fence;
+  // CE_DGRAD_ACC: ce_acc [M, N] fp32 = ce_acc * ce_accscale[row] + the piece's sum (null scale: = the sum)
+  float* ce_acc;
+  const float* ce_accscale;
 };
 // 256x256 8-phase pipelined GEMM (gemm8.hip); same epilogues.  a_t: A stored [K, M]; b_t: B stored
 // [K, N] (NN data-grad); both: TN weight-grad (use GEMM_EPI_F32ACC with gemm8_pick_ksplit / ws)
@@ -237,6 +242,24 @@ long lm_head_ce_ws_floats(int M, int Vpad, int K);
 // vocab splits of the CE dgrad for an M-row chunk (1 = one pass straight into dh)
 int ce_dgrad_splits(int M, int K, int Vpad);
 void lm_head_ce(const CeArgs& a, hipStream_t st);
+// The same loss swept in pieces of the vocabulary (ce_pieces.hip): no buffer grows with the vocabulary.
+struct CePiecesArgs {
+  const bf16_t* h; long ldh;   // [M, Kp] (Kp = K rounded up to 64, columns K .. Kp - 1 zeros)
+  const bf16_t* W; long ldw;   // [rows, Kp]-readable bf16 table, or null: the 4-bit one
+  long w_rows;                 // rows of W that may be read
+  const uint8_t *codes, *scales;  // the 4-bit table [V, K]
+  const int64_t* labels;       // [M]; outside [0, V): an ignored row
+  int M, K, Kp, V;
+  int piece;                   // columns of a full piece (% 256 == 0)
+  float* loss;                 // [1] mean over the valid rows (0 without any)
+  float* loss_rows;            // [M], 0 for ignored rows
+  int64_t* n_valid;            // [1]
+  bf16_t* dh;                  // [M, K] contiguous, null: loss only
+  void* ws;                    // lm_head_ce_pieces_ws_bytes
+};
+long lm_head_ce_pieces_ws_bytes(const CePiecesArgs& a);
+int lm_head_ce_pieces_width(long M, int V);  // the default piece
+void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st);
 // log-softmax gather: out[m, c] = logits[m, idx[c]] - lse(logits[m])  (MMLU scoring)
 void logsoftmax_gather(const bf16_t* logits, const int64_t* idx, float* out, long M, int V, long ld, int nidx,
                        hipStream_t st);

@@ -1,0 +1,337 @@
+// LM-head cross entropy swept in pieces of the vocabulary.
+//
+// One sweep, two products per piece of P columns:
+//   1. the logits product with the CE_FWD epilogue: E = exp(logit - tile max) in bf16 ([M, P], the only
+//      vocabulary-wide buffer), (max, sum) per row and 256-column tile, the label's logit;
+//   2. ce_piece_finalize: the running row maximum M' and sum S' over the pieces so far, the factor
+//      exp(M - M') that rescales what earlier pieces added, the dgrad's per-tile factors;
+//   3. the gradient product A' = A exp(M - M') + sum_v exp(l_v - M') W_v in fp32.
+// At the end, with lse = M + log S and p the label's probability,
+//   loss = lse - l_label,   dh = w (A / S - (1 - p) W_label),   w = 1 / valid rows,
+// the label's own column being left out of A (its E is set to 0): a row that is sure of its label has p near 1,
+// and (p - 1) W_label from a p rounded to bf16 would drown the small gradient that is left.
+// A 4-bit table is turned into bf16 one piece at a time, in a workspace of P rows.
+#include "common.h"
+#include "kernels.h"
+
+#include <algorithm>
+#include <cstdio>
+#include <cstdlib>
+
+namespace mft {
+
+namespace {
+
+// a row's position inside its 256-row tile in the order the CE dgrad reads its row factors (gemm8.hip)
+__device__ __forceinline__ long ratio_pos(int R) {
+  const int rl = R & 255;
+  return (R & ~255) + (rl >> 6) * 64 + (rl & 15) * 4 + ((rl >> 4) & 3);
+}
+
+// One workgroup: the valid rows counted, w = 1 / max(1, count), the running state cleared, the labels of the
+// first piece (relative to it, -100 elsewhere).
+__global__ __launch_bounds__(1024) void ce_pieces_begin_kernel(const int64_t* __restrict__ labels, int M, int V, int w0,
+                                                               int64_t* __restrict__ rel, float* __restrict__ run_m,
+                                                               float* __restrict__ run_s, float* __restrict__ lbl,
+                                                               float* __restrict__ zero, float* __restrict__ weight,
+                                                               int64_t* __restrict__ n_valid) {
+  __shared__ float red[16];
+  float n = 0.f;  // M < 2^24: exact in fp32
+  for (int i = threadIdx.x; i < M; i += 1024) {
+    const int64_t l = labels[i];
+    if (l >= 0 && l < V) n += 1.f;
+    rel[i] = l >= 0 && l < w0 ? l : -100;
+    run_m[i] = -INFINITY;
+    run_s[i] = 0.f;
+    lbl[i] = 0.f;
+    zero[i] = 0.f;
+  }
+  n = block_sum(n, red);
+  if (threadIdx.x == 0) {
+    *weight = 1.f / fmaxf(n, 1.f);
+    *n_valid = (int64_t)n;
+  }
+}
+
+// RB rows per block.  Pass 1 (a wave per row, lanes over the piece's tiles): the piece's maximum and sum join the
+// running ones.  Pass 2: ratio[t][row] = exp(m'_{t-1} - m'_t) with m'_t = max(m_t, M' - 60) -- a tile 60 below the
+// maximum adds less than e^-60, and the clamp keeps every factor and partial sum finite in fp32 -- staged through
+// LDS so that reads run over tiles and writes over rows.
+template <int RB>
+__global__ __launch_bounds__(256) void ce_piece_finalize_kernel(const float2* __restrict__ stats, int M, int T, long mpad,
+                                                                const int64_t* __restrict__ labels, int next0, int next_w,
+                                                                int64_t* __restrict__ rel, float* __restrict__ run_m,
+                                                                float* __restrict__ run_s, float* __restrict__ accscale,
+                                                                bf16_t* __restrict__ E, long lde,
+                                                                float* __restrict__ ratio, float* __restrict__ fin,
+                                                                int nsplit, int tps) {
+  __shared__ float s_mx[RB];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r0 = blockIdx.x * RB;
+  for (int rr = w; rr < RB; rr += 4) {
+    const int R = r0 + rr;
+    if (R >= M) break;
+    const float2* st = stats + (long)R * T;
+    float m = -INFINITY;
+    for (int t = lane; t < T; t += 64) m = fmaxf(m, st[t].x);
+    const float m0 = run_m[R];
+    m = fmaxf(wave_max(m), m0);
+    float s = 0.f;
+    for (int t = lane; t < T; t += 64) {
+      const float2 v = st[t];
+      s += v.y == 0.f ? 0.f : v.y * __expf(v.x - m);
+    }
+    s = wave_sum(s);
+    const float back = m0 == -INFINITY ? 0.f : __expf(m0 - m);
+    if (fin)
+      for (int sp = lane; sp < nsplit; sp += 64) {
+        const int te = min((sp + 1) * tps, T) - 1;
+        fin[(long)sp * M + R] = __expf(fmaxf(st[te].x, m - 60.f) - m);
+      }
+    if (lane == 0) {
+      s_mx[rr] = m;
+      run_m[R] = m;
+      run_s[R] = run_s[R] * back + s;
+      if (accscale) accscale[R] = back;
+      const int64_t here = rel[R];
+      if (E && here >= 0) E[(long)R * lde + here] = 0;
+      const int64_t l = labels[R];
+      rel[R] = l >= next0 && l < (int64_t)next0 + next_w ? l - next0 : -100;
+    }
+  }
+  if (!ratio || T < 2) return;
+  __shared__ float s_m[RB][65];
+  __syncthreads();
+  const int nrow = min(RB, M - r0);
+  const int rr2 = threadIdx.x % RB, jg = threadIdx.x / RB;
+  const long dst = ratio_pos(r0 + rr2);
+  for (int c0 = 0; c0 < T - 1; c0 += 63) {
+    const int cn = min(64, T - c0);
+    for (int rr = w; rr < nrow; rr += 4)
+      if (lane < cn) s_m[rr][lane] = fmaxf(stats[(long)(r0 + rr) * T + c0 + lane].x, s_mx[rr] - 60.f);
+    __syncthreads();
+    if (rr2 < nrow)
+      for (int j = 1 + jg; j < cn; j += 256 / RB) ratio[(long)(c0 + j) * mpad + dst] = __expf(s_m[rr2][j - 1] - s_m[rr2][j]);
+    __syncthreads();
+  }
+}
+
+// acc = acc * accscale[row] (absent on the first piece) + the split slabs in split order
+__global__ __launch_bounds__(256) void ce_piece_merge_kernel(const float* __restrict__ slab, int S, int M, int N,
+                                                             const float* __restrict__ accscale, float* __restrict__ acc) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4, MN = (long)M * N;
+  if (i >= MN) return;
+  f32x4_t a = *reinterpret_cast<const f32x4_t*>(slab + i);
+  for (int sp = 1; sp < S; ++sp) a += *reinterpret_cast<const f32x4_t*>(slab + sp * MN + i);
+  if (accscale) a += *reinterpret_cast<const f32x4_t*>(acc + i) * accscale[i / N];
+  *reinterpret_cast<f32x4_t*>(acc + i) = a;
+}
+
+// one 8-column piece of 4-bit values, as fp32
+__device__ __forceinline__ void mx4_load8(const uint8_t* codes, const uint8_t* scales, long row, int K, int c, float* f) {
+  typedef float f32x2v __attribute__((ext_vector_type(2)));
+  const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + row * (K / 2) + c / 2);
+  const uint32_t b = scales[row * (K / 32) + c / 32];
+  const float s = __uint_as_float(b == 255u ? 0x7fc00000u : b << 23);
+  const f32x2v v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 1),
+               v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3);
+  f[0] = v0[0], f[1] = v0[1], f[2] = v1[0], f[3] = v1[1], f[4] = v2[0], f[5] = v2[1], f[6] = v3[0], f[7] = v3[1];
+}
+
+// a wave per row: its loss and, with dh, its gradient
+__global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __restrict__ run_m, const float* __restrict__ run_s,
+                                                             const float* __restrict__ lbl, const int64_t* __restrict__ labels,
+                                                             int M, int K, int V, const float* __restrict__ weight,
+                                                             const float* __restrict__ acc, const bf16_t* __restrict__ W,
+                                                             long ldw, const uint8_t* __restrict__ codes,
+                                                             const uint8_t* __restrict__ scales, float* __restrict__ loss_rows,
+                                                             bf16_t* __restrict__ dh) {
+  const int R = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (R >= M) return;
+  const int64_t lab = labels[R];
+  const bool valid = lab >= 0 && lab < V;
+  const float s = run_s[R], lse = run_m[R] + __logf(s), nll = lse - lbl[R];
+  if (lane == 0) loss_rows[R] = valid ? nll : 0.f;
+  if (!dh) return;
+  const float wt = *weight, fa = wt / s, fl = wt * -expm1f(-nll);  // 1 - p = 1 - exp(l - lse)
+  for (int c = lane * 8; c < K; c += 512) {
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (valid) {
+      float wl[8];
+      if (W) load8(W + lab * ldw + c, wl);
+      else mx4_load8(codes, scales, lab, K, c, wl);
+      const float* a = acc + (long)R * K + c;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = a[j] * fa - wl[j] * fl;
+    }
+    store8(dh + (long)R * K + c, o);
+  }
+}
+
+// one workgroup, fixed order: loss = weight * sum of the rows' losses
+__global__ __launch_bounds__(1024) void ce_pieces_loss_kernel(const float* __restrict__ loss_rows, int M,
+                                                              const float* __restrict__ weight, float* __restrict__ loss) {
+  __shared__ float red[16];
+  float s = 0.f;
+  for (int i = threadIdx.x; i < M; i += 1024) s += loss_rows[i];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) *loss = s * *weight;
+}
+
+// rows of the operand copied with zero padding: out [rows, kpad], in [rows_in >= .., K] (ragged last piece)
+__global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict__ in, long ldi, long rows_in, int K,
+                                                       bf16_t* __restrict__ out, long rows, int kpad) {
+  const int k8 = kpad / 8;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * k8) return;
+  const long r = i / k8;
+  const int c = (int)(i - r * k8) * 8;
+  u16x8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (r < rows_in && c < K) v = *reinterpret_cast<const u16x8_t*>(in + r * ldi + c);
+  *reinterpret_cast<u16x8_t*>(out + r * kpad + c) = v;
+}
+
+int num_cus() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    MFT_HIP_CHECK(hipGetDevice(&dev));
+    MFT_HIP_CHECK(hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev));
+    return v > 0 ? v : 256;
+  }();
+  return n;
+}
+
+struct Layout {
+  float *run_m, *run_s, *lbl, *zero, *accscale, *weight, *stats, *ratio, *fin, *slab, *acc;
+  int64_t* rel;
+  bf16_t *E, *wb;
+  long bytes;
+};
+
+struct Plan {
+  int width;      // columns of a full piece, <= the padded vocabulary
+  int last;       // columns of the last piece
+  int n;          // pieces
+  int splits;     // of a full piece's dgrad
+  bool copy_all, copy_last;  // the table's pieces pass through the bf16 workspace
+};
+
+int up64(int x) { return (x + 63) / 64 * 64; }
+
+Plan make_plan(const CePiecesArgs& a) {
+  Plan p{};
+  p.width = std::min(a.piece, (a.V + 255) / 256 * 256);
+  p.n = (a.V + p.width - 1) / p.width;
+  p.last = a.V - (p.n - 1) * p.width;
+  p.copy_all = !a.W || a.K != a.Kp;
+  p.copy_last = p.copy_all || (long)(p.n - 1) * p.width + up64(p.last) > a.w_rows;
+  p.splits = a.dh ? ce_dgrad_splits(a.M, a.K, p.n > 1 ? p.width : up64(p.last)) : 1;
+  return p;
+}
+
+Layout make_layout(const CePiecesArgs& a, const Plan& p) {
+  const long M = a.M, T = p.width / 256, mpad = (M + 255) / 256 * 256;
+  // the last piece may split otherwise than the full ones
+  const long S = std::max(p.splits, a.dh ? ce_dgrad_splits(a.M, a.K, up64(p.last)) : 1);
+  Layout L{};
+  long o = 0;
+  char* base = reinterpret_cast<char*>(a.ws);
+  auto take = [&](long bytes) {
+    char* q = base ? base + o : nullptr;
+    o += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  auto floats = [&](long n) { return reinterpret_cast<float*>(take(n * 4)); };
+  L.run_m = floats(M), L.run_s = floats(M), L.lbl = floats(M), L.zero = floats(M), L.accscale = floats(M);
+  L.weight = floats(1);
+  L.rel = reinterpret_cast<int64_t*>(take(M * 8));
+  L.stats = floats(2 * M * T);
+  if (a.dh) {
+    L.ratio = floats(T * mpad);
+    L.fin = floats(S * M);
+    if (S > 1) L.slab = floats(S * M * a.K);
+    L.acc = floats(M * a.K);
+    L.E = reinterpret_cast<bf16_t*>(take(M * (long)p.width * 2));
+  }
+  if (p.copy_last) L.wb = reinterpret_cast<bf16_t*>(take((long)std::min(p.width, p.copy_all && p.n > 1 ? p.width : up64(p.last)) * a.Kp * 2));
+  L.bytes = o;
+  return L;
+}
+
+}  // namespace
+
+int lm_head_ce_pieces_width(long M, int V) {
+  // E [M, piece] bf16 of 512 MiB, at least 4,096 columns (fewer launches and longer reductions per piece)
+  const long w = (512L << 20) / (2 * std::max(M, 1L)) / 256 * 256;
+  return (int)std::min(std::max(w, 4096L), (long)(V + 255) / 256 * 256);
+}
+
+long lm_head_ce_pieces_ws_bytes(const CePiecesArgs& a) {
+  CePiecesArgs b = a;
+  b.ws = nullptr;
+  return make_layout(b, make_plan(b)).bytes;
+}
+
+void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
+  if (a.M <= 0) return;
+  const Plan p = make_plan(a);
+  const Layout L = make_layout(a, p);
+  const long mpad = (long)((a.M + 255) / 256) * 256;
+  const bool grad = a.dh != nullptr;
+  ce_pieces_begin_kernel<<<1, 1024, 0, st>>>(a.labels, a.M, a.V, p.n > 1 ? p.width : p.last, L.rel, L.run_m, L.run_s, L.lbl,
+                                             L.zero, L.weight, a.n_valid);
+  int rb = 64;
+  for (; rb > 16 && (a.M + rb - 1) / rb < 2 * num_cus(); rb /= 2) {}
+  for (int i = 0; i < p.n; ++i) {
+    const int v0 = i * p.width, w = i + 1 < p.n ? p.width : p.last, wp = up64(w), T = (wp + 255) / 256;
+    const bf16_t* W = a.W ? a.W + (long)v0 * a.ldw : nullptr;
+    long ldw = a.ldw;
+    if (p.copy_all || (p.copy_last && i + 1 == p.n)) {
+      if (a.W) {
+        const long n8 = (long)wp * (a.Kp / 8);
+        pad_rows_kernel<<<(unsigned)((n8 + 255) / 256), 256, 0, st>>>(W, a.ldw, w, a.K, L.wb, wp, a.Kp);
+      } else {
+        mx4_dequantize(a.codes, a.scales, v0, a.V, a.K, L.wb, a.Kp, wp, a.Kp, st);
+      }
+      W = L.wb;
+      ldw = a.Kp;
+    }
+    GemmArgs f{};
+    f.A = a.h; f.lda = a.ldh;
+    f.B = W; f.ldb = ldw;
+    f.C = grad ? L.E : nullptr; f.ldc = wp;
+    f.M = a.M; f.N = wp; f.K = a.Kp; f.alpha = 1.f;
+    f.ce_labels = L.rel; f.ce_stats = L.stats; f.ce_lbl = L.lbl; f.ce_V = w;
+    if (gemm4_supported(a.M, wp, a.Kp, false, false)) gemm4x(f, GEMM_EPI_CE_FWD, false, false, st);
+    else gemm8x(f, GEMM_EPI_CE_FWD, false, false, st);
+    const int S = grad ? ce_dgrad_splits(a.M, a.K, wp) : 1;
+    const int tps = S > 1 ? ((wp / 64 + S - 1) / S) / 4 : T;
+    auto fk = rb == 64 ? ce_piece_finalize_kernel<64> : rb == 32 ? ce_piece_finalize_kernel<32> : ce_piece_finalize_kernel<16>;
+    const int next0 = v0 + w, next_w = i + 1 >= p.n ? 0 : i + 2 < p.n ? p.width : p.last;
+    fk<<<(a.M + rb - 1) / rb, 256, 0, st>>>(reinterpret_cast<const float2*>(L.stats), a.M, T, mpad, a.labels, next0, next_w,
+                                            L.rel, L.run_m, L.run_s, grad ? L.accscale : nullptr, grad ? L.E : nullptr, wp,
+                                            L.ratio, L.fin, S, tps);
+    if (!grad) continue;
+    GemmArgs d{};
+    d.A = L.E; d.lda = wp;
+    d.B = W; d.ldb = ldw;
+    d.M = a.M; d.N = a.K; d.K = wp; d.alpha = 1.f;
+    d.ce_labels = L.rel; d.ce_ratio = L.ratio; d.ce_fin = L.fin; d.ce_wlab = L.zero;
+    if (S > 1) {
+      d.ksplit = S;
+      d.ws = L.slab;
+      gemm8x(d, GEMM_EPI_CE_DGRAD, false, true, st);
+      const long n4 = (long)a.M * a.K / 4;
+      ce_piece_merge_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(L.slab, S, a.M, a.K, i ? L.accscale : nullptr, L.acc);
+    } else {
+      d.ce_acc = L.acc;
+      d.ce_accscale = i ? L.accscale : nullptr;
+      gemm8x(d, GEMM_EPI_CE_DGRAD_ACC, false, true, st);
+    }
+  }
+  ce_pieces_rows_kernel<<<(a.M + 3) / 4, 256, 0, st>>>(L.run_m, L.run_s, L.lbl, a.labels, a.M, a.K, a.V, L.weight, L.acc, a.W,
+                                                       a.ldw, a.codes, a.scales, a.loss_rows, a.dh);
+  ce_pieces_loss_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.M, L.weight, a.loss);
+}
+
+}  // namespace mft

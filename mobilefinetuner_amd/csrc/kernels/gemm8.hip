@@ -44,6 +44,10 @@ namespace {
 constexpr int kHalf = 128 * 64;  // elements in a half-tile
 
 typedef __attribute__((address_space(3))) void lds_void8;
+// the two LM-head CE data gradients: straight into dh (or split slabs), and into a running fp32 sum
+template <int EPI>
+constexpr bool kCeDgrad = EPI == GEMM_EPI_CE_DGRAD || EPI == GEMM_EPI_CE_DGRAD_ACC;
+
 typedef const __attribute__((address_space(1))) void g_void8;
 
 __device__ __forceinline__ void glds16_8(const void* src, void* lds_wave_base) {
@@ -377,6 +381,52 @@ __device__ __forceinline__ void epilogue_ce_dgrad(const GemmArgs& g, f32x4_t (&a
   }
 }
 
+// CE_DGRAD_ACC (a piece of the vocabulary, one split): ce_acc[row][col] = ce_acc * ce_accscale[row] + fin * acc,
+// fp32; without ce_accscale (the first piece) a plain store.  Each element belongs to one workgroup.
+__device__ __forceinline__ void epilogue_ce_dgrad_acc(const GemmArgs& g, f32x4_t (&acc)[4][4][2], int m0, int n0, int wm,
+                                                      int wn, int lane) {
+  const int g4 = lane >> 4;
+  const int cofs = (g4 & 1) * 16 + (g4 >> 1) * 8;
+  float fin[2][4], old[2][4];
+#pragma unroll
+  for (int qa = 0; qa < 2; ++qa)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rr = min(m0 + qa * 128 + wm * 64 + i * 16 + (lane & 15), g.M - 1);
+      fin[qa][i] = g.ce_fin[rr];
+      old[qa][i] = g.ce_accscale ? g.ce_accscale[rr] : 0.f;
+    }
+#pragma unroll
+  for (int qa = 0; qa < 2; ++qa)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int q = qa ? (h ? 2 : 3) : (h ? 1 : 0);  // quadrant (qa, qb = h)
+      const int col = n0 + h * 128 + wn * 32 + cofs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float o[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[q][i][0][r]),
+                                                           __float_as_uint(acc[q][i][1][r]), false, false);
+          o[r] = __uint_as_float(sw[0]) * fin[qa][i];
+          o[4 + r] = __uint_as_float(sw[1]) * fin[qa][i];
+        }
+        const int row = m0 + qa * 128 + wm * 64 + i * 16 + (lane & 15);
+        if (col < g.N && row < g.M) {
+          f32x4_t* P = reinterpret_cast<f32x4_t*>(g.ce_acc + (long)row * g.N + col);
+          f32x4_t a = f32x4_t{o[0], o[1], o[2], o[3]}, b = f32x4_t{o[4], o[5], o[6], o[7]};
+          if (g.ce_accscale) {
+            a += P[0] * old[qa][i];
+            b += P[1] * old[qa][i];
+          }
+          P[0] = a;
+          P[1] = b;
+        }
+      }
+    }
+}
+
 // Workgroup barrier for an LDS exchange only: this wave's LDS operations retired, then a raw
 // s_barrier.  __syncthreads() is a workgroup fence as well, for which the compiler waits on
 // vmcnt(0) -- every global store still in flight (the CE forward's 128 KB tile of E) would stall
@@ -667,7 +717,7 @@ __device__ unsigned long long* g8_stamps;
 // KEEPB defaults on where the 16 extra VGPRs fit without spilling (not the TT wgrad form or the CE
 // dgrad, which spill 2-7 VGPRs with it; the LoRA epilogue fits since it walks the ranks 4 at a time)
 template <int EPI, bool AT, bool BT, bool LATE = true,
-          bool KEEPB = !(AT && BT) && EPI != GEMM_EPI_CE_DGRAD, bool LDSEPI = false>
+          bool KEEPB = !(AT && BT) && !kCeDgrad<EPI>, bool LDSEPI = false>
 __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   extern __shared__ __attribute__((aligned(16))) bf16_t smem[];
   if (g.stagger > 0 && blockIdx.x < 256) {  // first round: spread each XCD's CUs over a tile round
@@ -763,7 +813,7 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   // half-tiles at the phase-8 vm_wait, so the counted waits retire it with no extra wait.
   float* const rslot = reinterpret_cast<float*>(smem + 8 * kHalf);
   auto ce_dma = [&](int kt) {
-    if constexpr (EPI == GEMM_EPI_CE_DGRAD) {
+    if constexpr (kCeDgrad<EPI>) {
       const int tt = kt / 4 + 1;  // local vocab tile of this split (kbase is a whole number of tiles)
       if ((kt & 3) == 0 && tt * 4 < nk && w == 0) {
         const long mpad = (long)((g.M + 255) / 256) * 256;
@@ -773,7 +823,7 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   };
   // the phase's 4 row factors: read with its fragments (before lds_sync), applied after it
   auto ce_read = [&](int q, int kt) -> f32x4_t {
-    if constexpr (EPI == GEMM_EPI_CE_DGRAD) {
+    if constexpr (kCeDgrad<EPI>) {
       if ((kt & 3) == 0 && kt > 0)
         return *reinterpret_cast<const f32x4_t*>(rslot + ((kt / 4) & 1) * 256 + (q < 2 ? 0 : 128) + wm * 64 +
                                                  (lane & 15) * 4);
@@ -787,7 +837,7 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   // second MFMA code path for the tile starts spills.  Scalar asm multiplies: left to the
   // compiler they become v_pk_mul_f32, which costs extra cycles beside MFMAs.
   auto mma_ce = [&](int q, const f32x4_t& r) {
-    if constexpr (EPI == GEMM_EPI_CE_DGRAD) {
+    if constexpr (kCeDgrad<EPI>) {
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
@@ -833,7 +883,7 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   // workgroup-uniform branch; staging and the counted waits are unchanged).  Not in the CE dgrad:
   // there the three column tiles of a row block stream the same 34 GB E operand in lockstep through
   // L2, and a faster third tile breaks that sharing (measured 21.9 -> 23.2 ms at Gemma-3's shape).
-  const bool b1_ok = EPI == GEMM_EPI_CE_DGRAD || g.ntail_full || n0 + 128 < g.N;
+  const bool b1_ok = kCeDgrad<EPI> || g.ntail_full || n0 + 128 < g.N;
 
   // a phase's first barrier: fragment-read wait before (default) or after (LATE) it
   auto pre_sync = [&]() {
@@ -935,7 +985,8 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
     if constexpr (LDSEPI) raw_barrier();  // every wave's tail LDS-DMA retired before the image overwrites LDS
     epilogue_ce_fwd<LDSEPI>(g, acc, m0, n0, wm, wn, lane, reinterpret_cast<float*>(smem));
   }
-  else if constexpr (EPI == GEMM_EPI_CE_DGRAD) epilogue_ce_dgrad(g, acc, m0, n0, wm, wn, lane, split);
+  else if constexpr (EPI == GEMM_EPI_CE_DGRAD_ACC) epilogue_ce_dgrad_acc(g, acc, m0, n0, wm, wn, lane);
+  else if constexpr (kCeDgrad<EPI>) epilogue_ce_dgrad(g, acc, m0, n0, wm, wn, lane, split);
   else if constexpr (LDSEPI && (EPI == GEMM_EPI_NONE || EPI == GEMM_EPI_BIAS || EPI == GEMM_EPI_BIAS_GELU_D ||
                                  EPI == GEMM_EPI_DGELU || EPI == GEMM_EPI_MUL_AUX)) {
     raw_barrier();  // every wave's tail LDS-DMA retired (vm_wait<0> above) before the tile overwrites LDS
@@ -1419,7 +1470,7 @@ static int gemm8_stagger() {
 template <int EPI, bool AT, bool BT>
 static void launch8(const GemmArgs& g, hipStream_t st) {
   // 128 KB of half-tile buffers (+ 2 KB of row-factor slots for the CE dgrad)
-  constexpr size_t shm = sizeof(bf16_t) * 8 * kHalf + (EPI == GEMM_EPI_CE_DGRAD ? 2048 : 0);
+  constexpr size_t shm = sizeof(bf16_t) * 8 * kHalf + (kCeDgrad<EPI> ? 2048 : 0);
   static bool attr = false;
   if (!attr) {
     MFT_HIP_CHECK(hipFuncSetAttribute((const void*)gemm8_kernel<EPI, AT, BT>,
@@ -1441,7 +1492,7 @@ static void launch8(const GemmArgs& g, hipStream_t st) {
       return;
     }
   }
-  if constexpr (EPI != GEMM_EPI_CE_FWD && EPI != GEMM_EPI_CE_DGRAD) {
+  if constexpr (EPI != GEMM_EPI_CE_FWD && !kCeDgrad<EPI>) {
     if (gemm8_p2()) {
       static bool attr_p = false;
       if (!attr_p) {
@@ -1618,6 +1669,13 @@ void gemm8x(const GemmArgs& g0, int epi, bool a_t, bool b_t, hipStream_t st) {
         abort();
       }
       launch8<GEMM_EPI_CE_DGRAD, false, true>(g, st);
+      break;
+    case GEMM_EPI_CE_DGRAD_ACC:
+      if (a_t || !b_t || g.ksplit > 1 || !g.ce_ratio || !g.ce_fin || !g.ce_acc) {
+        fprintf(stderr, "mft::gemm8: the accumulating CE dgrad needs the NN layout, ratio/fin/acc and one split\n");
+        abort();
+      }
+      launch8<GEMM_EPI_CE_DGRAD_ACC, false, true>(g, st);
       break;
     default: fprintf(stderr, "mft::gemm8: bad epilogue %d\n", epi); abort();
   }

@@ -1143,9 +1143,50 @@ def lm_head_cross_entropy(h, w, labels, vocab_size, chunk=None, w_grad_scale=1.0
     which the NN dgrad consumes once with a per-tile accumulator rescale (see ``_LMHeadCE``).
     NOTE: the W gradient is produced during forward and scaled by ``w_grad_scale`` (pass the
     same factor the loss is later multiplied by, e.g. 1/grad_accum); dh honours grad_output."""
+    if isinstance(w, MX4Weight):
+        return lm_head_cross_entropy_pieces(h, w, labels, vocab_size)
     if chunk is None:
         chunk = default_ce_chunk(cw(w).shape[0])
     return _LMHeadCE.apply(h, w, labels, int(vocab_size), int(chunk), float(w_grad_scale))
+
+
+class _LMHeadCEPieces(Function):
+    """The loss and -- in the same sweep over the vocabulary -- dh (kernels/ce_pieces.hip); the backward pass
+    multiplies dh by the loss's gradient."""
+
+    @staticmethod
+    def forward(ctx, h, w, labels, V, piece):
+        loss, dh = _ce_pieces(h, w, labels, V, piece, ctx.needs_input_grad[0])
+        ctx.save_for_backward(dh)
+        return loss
+
+    @staticmethod
+    def backward(ctx, gout):
+        (dh,) = ctx.saved_tensors
+        return native().scale_bf16(dh, gout.float().reshape(1), 1.0), None, None, None, None
+
+
+def _ce_pieces(h, w, labels, V, piece, grad):
+    mx = isinstance(w, MX4Weight)
+    loss, _, _, dh = native().lm_head_ce_pieces(h, None if mx else cw(w), w.codes if mx else None, w.scales if mx else None,
+                                                labels.reshape(-1), V, piece, grad)
+    return loss, dh
+
+
+@_device_op
+def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
+    """Mean token NLL of logits = h W^T over the rows whose label lies in [0, vocab_size) (others, -100 among
+    them, are ignored; none at all gives 0), swept in pieces of ``piece`` vocabulary columns (a multiple of
+    256; None: a size from the row count): beside h, dh and an fp32 dh the memory is one [rows, piece] bf16
+    buffer, whatever the vocabulary -- lm_head_cross_entropy keeps one of the whole vocabulary's width.  W is
+    frozen: bf16 [>= vocab_size, C] (C a multiple of 8; padding rows, read up to the next multiple of 64, must be
+    finite) or an MX4Weight; the gradient goes to h.  A trainable W is lm_head_cross_entropy's."""
+    if _needs(w):
+        raise RuntimeError("lm_head_cross_entropy_pieces: W is frozen here; lm_head_cross_entropy trains it")
+    piece = int(piece or 0)
+    if torch.is_grad_enabled() and h.requires_grad:
+        return _LMHeadCEPieces.apply(h, w, labels, int(vocab_size), piece)
+    return _ce_pieces(h, w, labels, int(vocab_size), piece, False)[0]
 
 
 @_device_op
@@ -1153,6 +1194,9 @@ def lm_head_token_nll(h, w, labels, vocab_size, chunk=None):
     """Per-row NLL (no grad) for evaluation: returns (sum_nll, n_valid) device scalars."""
     with torch.no_grad():
         C = native()
+        if isinstance(w, MX4Weight):
+            _, rows, n, _ = C.lm_head_ce_pieces(h, None, w.codes, w.scales, labels.reshape(-1), int(vocab_size), 0, False)
+            return rows.sum(), n
         wc = cw(w)
         M = h.shape[0]
         if chunk is None:

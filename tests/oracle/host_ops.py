@@ -146,3 +146,11 @@ def lm_head_token_nll(h, w, labels, vocab_size, chunk=None):
         logits = (h.float() @ _w(w).float().t())[:, :vocab_size]
         nll = torch.nn.functional.cross_entropy(logits, labels.reshape(-1), ignore_index=-100, reduction="sum")
         return nll, (labels >= 0).sum()
+
+
+def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
+    labels = labels.reshape(-1)
+    labels = torch.where((labels >= 0) & (labels < vocab_size), labels, -100)
+    if not (labels >= 0).any():
+        return h.float().sum() * 0.0
+    return lm_head_cross_entropy(h, w, labels, vocab_size)

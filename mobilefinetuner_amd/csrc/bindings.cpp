@@ -325,14 +325,15 @@ std::pair<long, int> mx4_shape(const Tensor& codes, const Tensor& scales, const 
                   scales.dim() == 2 && codes.is_contiguous() && scales.is_contiguous(),
               what, ": codes and scales must be contiguous 2-D uint8 tensors");
   const long N = codes.size(0), K = codes.size(1) * 2;
-  TORCH_CHECK(K > 0 && K % 32 == 0 && K <= 0x3fffffff && N <= 0x3fffffff && scales.size(0) == N && scales.size(1) == K / 32, what,
+  TORCH_CHECK(K > 0 && K % 32 == 0 && scales.size(0) == N && scales.size(1) == K / 32, what,
               ": codes [N, K / 2] with K % 32 == 0 and scales [N, K / 32]");
+  TORCH_CHECK(K < (1 << 22) && N < (1 << 22), what, ": at most 2^22 - 1 rows and columns");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, what, ": codes must start at a 16-byte boundary");
   return {N, (int)K};
 }
 const uint8_t* u8p(const Tensor& t) { return t.data_ptr<uint8_t>(); }
-bool rows16(const Tensor& t) {  // 2-D bf16 rows that 16-byte loads may walk
-  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+bool rows16(const Tensor& t) {  // 2-D bf16 rows that 16-byte loads may walk, apart by less than 2^22 elements
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) < (1 << 22) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
 std::vector<Tensor> mx4_quantize(Tensor w) {
@@ -340,7 +341,7 @@ std::vector<Tensor> mx4_quantize(Tensor w) {
   const bool f32 = w.scalar_type() == torch::kFloat32;
   TORCH_CHECK(f32 || w.scalar_type() == torch::kBFloat16, "mx4_quantize: W must be fp32 or bf16");
   TORCH_CHECK(w.dim() == 2 && w.size(1) > 0 && w.size(1) % 32 == 0, "mx4_quantize: W [N, K] with K a multiple of 32");
-  TORCH_CHECK(w.size(0) <= 0x3fffffff && w.size(1) <= 0x3fffffff, "mx4_quantize: W has too many rows or columns");
+  TORCH_CHECK(w.size(0) < (1 << 22) && w.size(1) < (1 << 22), "mx4_quantize: at most 2^22 - 1 rows and columns");
   c10::DeviceGuard g(w.device());
   w = w.contiguous();
   if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) w = w.clone();
@@ -415,8 +416,17 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   a.bias = optp<bf16_t>(bias);
   a.y = bp(y); a.ldy = out;
   a.M = (int)x2.size(0); a.N = (int)N; a.K = K;
-  if (dgrad) mft::mx4_dgrad(a, stream());
-  else mft::mx4_linear(a, stream());
+  if (!dgrad && a.M <= 64) {
+    mft::mx4_rows(a, stream());
+    return y;
+  }
+  const auto plan = mft::mx4_plan(a.M, a.N, a.K, dgrad);
+  Tensor ws;
+  if (const long n = mft::mx4_plan_ws_floats(plan, a.M, a.N, a.K, dgrad)) {
+    ws = torch::empty({n}, x.options().dtype(torch::kFloat32));
+    a.ws = fp(ws);
+  }
+  mft::mx4_tiles(a, plan, dgrad, stream());
   return y;
 }
 Tensor mx4_linear(Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> bias) {

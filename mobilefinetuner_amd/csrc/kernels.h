@@ -401,9 +401,15 @@ struct Mx4LinearArgs {
   bf16_t* y;        // linear: y [M, N]; dgrad: dx [M, K] (ldy % 4 == 0, 8-B aligned)
   long ldy;
   int M, N, K;
+  float* ws;  // mx4_plan_ws_floats
 };
-void mx4_linear(const Mx4LinearArgs& a, hipStream_t st);  // y = x W^T + bias
-void mx4_dgrad(const Mx4LinearArgs& a, hipStream_t st);   // dx = dy W
+void mx4_rows(const Mx4LinearArgs& a, hipStream_t st);  // y = x W^T + bias, M <= 64 (mx4.hip)
+struct Mx4Plan {
+  int bm, tn, splits;  // rows and 64-column strips of a tile, workgroups that share a tile's reduction
+};
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad);
+long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad);
+void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);  // y, or dx = dy W (mx4_gemm.hip)
 
 // ---------------------------------------------------------------- misc (misc.hip)
 void cast_f32_bf16(const float* x, bf16_t* y, long n, hipStream_t st);

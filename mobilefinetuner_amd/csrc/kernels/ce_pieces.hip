@@ -13,6 +13,7 @@
 // A 4-bit table is turned into bf16 one piece at a time, in a workspace of P rows.
 #include "common.h"
 #include "kernels.h"
+#include "mx4.h"
 
 #include <algorithm>
 #include <cstdio>
@@ -127,17 +128,6 @@ __global__ __launch_bounds__(256) void ce_piece_merge_kernel(const float* __rest
   *reinterpret_cast<f32x4_t*>(acc + i) = a;
 }
 
-// one 8-column piece of 4-bit values, as fp32
-__device__ __forceinline__ void mx4_load8(const uint8_t* codes, const uint8_t* scales, long row, int K, int c, float* f) {
-  typedef float f32x2v __attribute__((ext_vector_type(2)));
-  const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + row * (K / 2) + c / 2);
-  const uint32_t b = scales[row * (K / 32) + c / 32];
-  const float s = __uint_as_float(b == 255u ? 0x7fc00000u : b << 23);
-  const f32x2v v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 1),
-               v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, s, 3);
-  f[0] = v0[0], f[1] = v0[1], f[2] = v1[0], f[3] = v1[1], f[4] = v2[0], f[5] = v2[1], f[6] = v3[0], f[7] = v3[1];
-}
-
 // a wave per row: its loss and, with dh, its gradient
 __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __restrict__ run_m, const float* __restrict__ run_s,
                                                              const float* __restrict__ lbl, const int64_t* __restrict__ labels,
@@ -159,7 +149,11 @@ __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __rest
     if (valid) {
       float wl[8];
       if (W) load8(W + lab * ldw + c, wl);
-      else mx4_load8(codes, scales, lab, K, c, wl);
+      else {
+        const bf16x8_t v = mx4_cvt8(*reinterpret_cast<const uint32_t*>(codes + lab * (K / 2) + c / 2), mx4_scale(scales[lab * (K / 32) + c / 32]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wl[j] = (float)v[j];
+      }
       const float* a = acc + (long)R * K + c;
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = a[j] * fa - wl[j] * fl;

@@ -8,7 +8,7 @@
 // largest 6 * 2^125 (finite).
 #include "common.h"
 #include "kernels.h"
-#include "mfma.h"
+#include "mx4.h"
 
 #include <cstdio>
 #include <cstdlib>
@@ -16,21 +16,6 @@
 namespace mft {
 
 namespace {
-
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
-
-// scale byte -> the fp32 whose exponent field it is; 255 -> NaN
-__device__ __forceinline__ float mx4_scale(uint32_t byte) {
-  return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
-}
-
-// 8 codes (one 32-bit word, low half-byte first) -> 8 bf16 values
-__device__ __forceinline__ bf16x8_t mx4_cvt8(uint32_t w, float s) {
-  const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1),
-                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
-  return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // ------------------------------------------------------------------ quantise
 // Four lanes share a group of 32 columns (8 each).  The scale: with a = max |w| = f 2^e, 1 <= f < 2, the
@@ -110,124 +95,117 @@ __global__ __launch_bounds__(256) void mx4_embed_kernel(const int64_t* __restric
   store8(out + m * K + c8 * 8, f);
 }
 
-// ------------------------------------------------------------------ y = x W^T + b, rows by rows
-// A wave owns 16 output columns (rows n of W) and MT * 16 rows of x.  Per 128 columns of K a lane loads 16 B
+// ------------------------------------------------------------------ y = x W^T + b, few rows
+// A wave owns TN * 16 output columns (rows n of W) and MT * 16 rows of x.  Per 128 columns of K a lane loads 16 B
 // of codes -- one scale group -- of row n = n0 + (l & 15), columns 32 (l >> 4) .. + 31, and turns it into the
 // operands of four 16x16x32 MFMAs; step t multiplies columns 32 (l >> 4) + 8 t + j, so x is read with the
-// same permutation.  S waves of a workgroup share a column tile and split K; they meet in LDS.
-template <int MT, int S>
+// same permutation.  Nothing is staged: codes and x go from memory into the operands, the loads of U such
+// chunks in flight together.  S waves of a workgroup share a column tile and split K; they meet in LDS.
+template <int MT, int TN, int S, int U>
 __global__ __launch_bounds__(64 * (S > 4 ? S : 4)) void mx4_rows_kernel(Mx4LinearArgs g) {
-  constexpr int NW = S > 4 ? S : 4, TPB = NW / S;  // waves, column tiles per workgroup
-  __shared__ float red[S > 1 ? NW * MT * 256 : 1];
+  constexpr int NW = S > 4 ? S : 4, TPB = NW / S;  // waves, column tiles (of TN * 16) per workgroup
+  __shared__ float red[S > 1 ? NW * MT * TN * 256 : 1];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ks = w % S, r16 = lane & 15, kq = lane >> 4;
-  const int n0 = (blockIdx.x * TPB + w / S) * 16, m0 = blockIdx.y * (MT * 16);
-  const int n = min(n0 + r16, g.N - 1);
-  const uint4* crow = reinterpret_cast<const uint4*>(g.codes + (long)n * (g.K / 2));
-  const uint8_t* srow = g.scales + (long)n * (g.K / 32);
+  const int n0 = (blockIdx.x * TPB + w / S) * (16 * TN);
+  const int ng = g.K / 32;  // groups of a row; chunk c holds groups 4 c .. 4 c + 3
+  const uint4* crow[TN];
+  const uint8_t* srow[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = min(n0 + j * 16 + r16, g.N - 1);
+    crow[j] = reinterpret_cast<const uint4*>(g.codes + (long)n * (g.K / 2));
+    srow[j] = g.scales + (long)n * ng;
+  }
   const bf16_t* xrow[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) xrow[i] = g.x + (long)min(m0 + i * 16 + r16, g.M - 1) * g.ldx;
-  const int ng = g.K / 32;  // groups of a row; chunk c holds groups 4 c .. 4 c + 3
-  f32x4_t acc[MT];
+  for (int i = 0; i < MT; ++i) xrow[i] = g.x + (long)min(i * 16 + r16, g.M - 1) * g.ldx;
+  f32x4_t acc[MT][TN];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = zero4();
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = zero4();
   if (n0 < g.N) {
-    for (int c = ks; c * 4 < ng; c += S) {
-      const int grp = c * 4 + kq;
-      const bool in = grp < ng;
-      uint4 q = {0, 0, 0, 0};
-      float s = 1.f;
-      if (in) q = crow[grp], s = mx4_scale(srow[grp]);
-      const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+    for (int c = ks; c * 4 < ng; c += S * U) {
+      uint4 q[U][TN];
+      uint32_t sb[U][TN];
+      bf16x8_t a[U][MT][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bf16x8_t b = mx4_cvt8(qw[t], s);
+      for (int u = 0; u < U; ++u) {
+        // lanes past the row's end multiply zeros by zeros (their loads go to the last group)
+        const int grp = (c + u * S) * 4 + kq, gc = min(grp, ng - 1);
+        const bool in = grp < ng;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          bf16x8_t a = {};
-          if (in) a = *reinterpret_cast<const bf16x8_t*>(xrow[i] + grp * 32 + t * 8);
-          acc[i] = mfma16(b, a, acc[i]);  // C^T: lane holds columns n0 + 4 kq + r of row m0 + 16 i + r16
+        for (int j = 0; j < TN; ++j) {
+          q[u][j] = crow[j][gc];
+          sb[u][j] = srow[j][gc];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) a[u][i][t] = *reinterpret_cast<const bf16x8_t*>(xrow[i] + gc * 32 + t * 8);
+        if (!in) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) q[u][j] = uint4{0, 0, 0, 0}, sb[u][j] = 127;
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) a[u][i][t] = bf16x8_t{};
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const float s = mx4_scale(sb[u][j]);
+          const uint32_t qw[4] = {q[u][j].x, q[u][j].y, q[u][j].z, q[u][j].w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const bf16x8_t b = mx4_cvt8(qw[t], s);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)  // C^T: lane holds columns 16 j + 4 kq + r of row 16 i + r16
+              acc[i][j] = mfma16(b, a[u][i][t], acc[i][j]);
+          }
         }
       }
     }
   }
   if constexpr (S > 1) {
-    f32x4_t* p = reinterpret_cast<f32x4_t*>(red) + (long)w * MT * 64 + lane;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) p[i * 64] = acc[i];
-    __syncthreads();
-    if (ks != 0) return;
+    // wave ks of a tile sums every S-th accumulator block over the tile's waves, in wave order, and stores it
+    f32x4_t* p = reinterpret_cast<f32x4_t*>(red) + (w - ks) * (MT * TN * 64) + lane;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
-      for (int k = 1; k < S; ++k) acc[i] += p[(k * MT + i) * 64];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) p[(ks * MT * TN + i * TN + j) * 64] = acc[i][j];
+    __syncthreads();
   }
   if (n0 >= g.N) return;
-  const int nc = n0 + 4 * kq;
-  float bias[4] = {0.f, 0.f, 0.f, 0.f};
-  if (g.bias)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (nc + r < g.N) bias[r] = bf2f(g.bias[nc + r]);
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + i * 16 + r16;
-    if (m >= g.M) continue;
-    bf16_t* y = g.y + (long)m * g.ldy + nc;
+    for (int j = 0; j < TN; ++j) {
+      f32x4_t v = acc[i][j];
+      if constexpr (S > 1) {
+        if ((i * TN + j) % S != ks) continue;
+        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(red) + (w - ks) * (MT * TN * 64) + (i * TN + j) * 64 + lane;
+        v = p[0];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (nc + r < g.N) y[r] = f2bf(acc[i][r] + bias[r]);
-  }
-}
-
-// ------------------------------------------------------------------ dx = dy W
-// 64 rows x 128 columns per workgroup, 32 rows n of W per step: the workgroup turns the [32, 128] codes into a
-// bf16 LDS image and reads it transposed (ds_read_b64_tr_b16), dy comes straight from memory.
-constexpr int kDgLd = 128 + 8;
-__global__ __launch_bounds__(256) void mx4_dgrad_kernel(Mx4LinearArgs g) {
-  __shared__ __attribute__((aligned(16))) bf16_t img[32 * kDgLd];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
-  const int k0 = blockIdx.x * 128, m0 = blockIdx.y * 64;
-  const int pr = threadIdx.x >> 3, pc = (threadIdx.x & 7) * 16;  // this thread's 16 codes of the step's image
-  const bool pin = k0 + pc < g.K;
-  f32x4_t acc[4][2];
+        for (int k = 1; k < S; ++k) v += p[k * MT * TN * 64];
+      }
+      const int m = i * 16 + r16, nc = n0 + j * 16 + 4 * kq;
+      if (m >= g.M || nc >= g.N) continue;
+      bf16_t* y = g.y + (long)m * g.ldy + nc;
+      if (nc + 4 <= g.N && g.ldy % 4 == 0) {  // 8-byte rows and columns
+        if (g.bias) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = zero4();
-  for (int n0 = 0; n0 < g.N; n0 += 32) {
-    uint2 q = {0, 0};
-    float s = 1.f;
-    const int n = n0 + pr;
-    if (n < g.N && pin) {
-      q = *reinterpret_cast<const uint2*>(g.codes + (long)n * (g.K / 2) + (k0 + pc) / 2);
-      s = mx4_scale(g.scales[(long)n * (g.K / 32) + (k0 + pc) / 32]);
+          for (int r = 0; r < 4; ++r) v[r] += bf2f(g.bias[nc + r]);
+        }
+        *reinterpret_cast<uint2*>(y) = uint2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (nc + r < g.N) y[r] = f2bf(v[r] + (g.bias ? bf2f(g.bias[nc + r]) : 0.f));
+      }
     }
-    __syncthreads();
-    *reinterpret_cast<bf16x8_t*>(img + pr * kDgLd + pc) = mx4_cvt8(q.x, s);
-    *reinterpret_cast<bf16x8_t*>(img + pr * kDgLd + pc + 8) = mx4_cvt8(q.y, s);
-    __syncthreads();
-    const bf16x8_t b0 = frag_tr(img, kDgLd, 0, w * 32), b1 = frag_tr(img, kDgLd, 0, w * 32 + 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = min(m0 + i * 16 + r16, g.M - 1);
-      bf16x8_t a = {};
-      if (n0 + kq * 8 < g.N) a = *reinterpret_cast<const bf16x8_t*>(g.x + (long)m * g.ldx + n0 + kq * 8);
-      acc[i][0] = mfma16(b0, a, acc[i][0]);
-      acc[i][1] = mfma16(b1, a, acc[i][1]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + i * 16 + r16;
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int c = k0 + w * 32 + j * 16 + 4 * kq;
-      if (c >= g.K) continue;
-      u16x4_t v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = f2bf(acc[i][j][r]);
-      *reinterpret_cast<u16x4_t*>(g.y + (long)m * g.ldy + c) = v;
-    }
-  }
 }
 
 void check_grid(long blocks, const char* what) {
@@ -265,17 +243,35 @@ void mx4_embed(const int64_t* ids, const uint8_t* codes, const uint8_t* scales, 
                                                      S, scale);
 }
 
-void mx4_linear(const Mx4LinearArgs& a, hipStream_t st) {
-  if (a.M <= 0 || a.N <= 0) return;
-  const int tiles = (a.N + 15) / 16;
-  const dim3 grid1(tiles, (a.M + 15) / 16), grid4(tiles, (a.M + 63) / 64);
-  if (a.M <= 16) mx4_rows_kernel<1, 4><<<grid1, 256, 0, st>>>(a);
-  else mx4_rows_kernel<4, 4><<<grid4, 256, 0, st>>>(a);
+template <int MT, int TN, int S, int U>
+static void launch_rows(const Mx4LinearArgs& a, hipStream_t st) {
+  const int per = 16 * TN * (S > 4 ? 1 : 4 / S);
+  mx4_rows_kernel<MT, TN, S, U><<<(a.N + per - 1) / per, 64 * (S > 4 ? S : 4), 0, st>>>(a);
 }
 
-void mx4_dgrad(const Mx4LinearArgs& a, hipStream_t st) {
-  if (a.M <= 0 || a.K <= 0) return;
-  mx4_dgrad_kernel<<<dim3((a.K + 127) / 128, (a.M + 63) / 64), 256, 0, st>>>(a);
+// waves that split K, from the waves that the column tiles alone give
+template <int MT>
+static void launch_rows_mt(const Mx4LinearArgs& a, hipStream_t st) {
+  const int tiles = (a.N + 15) / 16, chunks = (a.K + 127) / 128;
+  const int force = getenv("MX4_S") ? atoi(getenv("MX4_S")) : 0;
+  int S = 1;
+  while (S < 16 && S < chunks && (long)tiles * S < 4096) S *= 2;
+  if (force) S = force;
+  constexpr int U = MT == 1 ? 2 : 1;
+  switch (S) {
+    case 1: launch_rows<MT, 2, 1, U>(a, st); break;
+    case 2: launch_rows<MT, 1, 2, U>(a, st); break;
+    case 4: launch_rows<MT, 1, 4, U>(a, st); break;
+    case 8: launch_rows<MT, 1, 8, U>(a, st); break;
+    default: launch_rows<MT, 1, 16, U>(a, st); break;
+  }
+}
+
+void mx4_rows(const Mx4LinearArgs& a, hipStream_t st) {
+  if (a.M <= 16) launch_rows_mt<1>(a, st);
+  else if (a.M <= 32) launch_rows_mt<2>(a, st);
+  else if (a.M <= 48) launch_rows_mt<3>(a, st);
+  else launch_rows_mt<4>(a, st);
 }
 
 }  // namespace mft

@@ -410,6 +410,9 @@ struct Mx4Plan {
 Mx4Plan mx4_plan(int M, int N, int K, bool dgrad);
 long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad);
 void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);  // y, or dx = dy W (mx4_gemm.hip)
+// the same through a bf16 copy of W (W^T for dx) in w [N * K] and gemm4
+bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx);
+void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st);
 
 // ---------------------------------------------------------------- misc (misc.hip)
 void cast_f32_bf16(const float* x, bf16_t* y, long n, hipStream_t st);

@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
+#include <type_traits>
 
 namespace mft {
 
@@ -30,17 +31,26 @@ __device__ __forceinline__ void glds16(const void* src, void* lds_wave_base) {
   __builtin_amdgcn_global_load_lds((glb_void*)src, (lds_void*)lds_wave_base, 16, 0, 0);
 }
 
-// every load of this wave arrived (LDS ones included), every LDS write of it done; then the workgroup's barrier
+// every load of this wave arrived (those to LDS included), every LDS access of it done; then the workgroup's barrier
 __device__ __forceinline__ void arrive() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <int BM, int TN, bool DG>
 constexpr int lds_bytes() {
-  return DG ? 2 * (BM * 128 + 64 * (32 * TN + 16) + 64 * 4 * 2 * TN) : 2 * BM * 256;
+  return 2 * (DG ? BM * 128 + 64 * (32 * TN + 16) + 64 * 4 * 2 * TN : BM * 256);
 }
 
-template <int BM, int TN, bool DG, bool PART>
+// Scale bytes travel as unaligned 32-bit words of four neighbouring groups, the byte taken at its use: a byte kept in
+// a register across steps is masked to 8 bits by the compiler right after its load, and that waits for every load
+// in flight.  NARROW: rows of fewer than four groups (K < 128), byte loads.
+__device__ __forceinline__ uint32_t load_u32(const uint8_t* p) {
+  uint32_t v;
+  __builtin_memcpy(&v, p, 4);
+  return v;
+}
+
+template <int BM, int TN, bool DG, bool PART, bool NARROW>
 __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int splits) {
   constexpr int MI = BM / 16, BN = 64 * TN;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -95,7 +105,7 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
   // T sub-steps of 32 reduction columns, each MI x TN MFMAs, in blocks of HB row tiles: while a block multiplies, the
   // next one's activation operands are read, and in a sub-step's last block the next sub-step's weight operands are
   // converted (conv(b, t)).  The scheduling barriers keep the compiler from pulling each read down to its first use.
-  constexpr int HB = MI < 4 ? MI : 4, T = STEP / 32, NB = T * MI / HB;
+  constexpr int HB = MI < 4 || (!DG && MI * TN == 32) ? 2 : 4, T = STEP / 32, NB = T * MI / HB;  // (128 x 256: 4 would spill)
   auto frag_a = [&](int buf, int i, int t) {
     const int row = i * 16 + r16;
     return *reinterpret_cast<const bf16x8_t*>(abuf(buf) + (row * CPR + ((t * 4 + kq) ^ swz(row))) * 8);
@@ -129,84 +139,88 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
     const uint8_t* sbp = g.scales + (long)c0 * ng;
     const int nlast = g.N - 1 - c0, nfirst = w * TN * 16 + r16, kb = g.K / 2;
     uint4 q[TN], qn[TN];
-    uint32_t sb[TN], sbn[TN];
+    uint32_t sw[TN], swn[TN];
     auto load_w = [&](uint4 (&qq)[TN], uint32_t (&ss)[TN], int s) {
-      const int grp = s * 4 + kq, gc = min(grp, ng - 1);
+      const int gc = min(s * 4 + kq, ng - 1);
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = min(nfirst + j * 16, nlast);
         qq[j] = *reinterpret_cast<const uint4*>(cb + (uint32_t)(__mul24(n, kb) + gc * 16));
-        ss[j] = sbp[(uint32_t)(__mul24(n, ng) + gc)];
+        if constexpr (NARROW) ss[j] = sbp[(uint32_t)(__mul24(n, ng) + gc)];
+        else ss[j] = load_u32(sbp + (uint32_t)(__mul24(n, ng) + min(s * 4, ng - 4)));
       }
-      if (grp >= ng) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) qq[j] = uint4{0, 0, 0, 0}, ss[j] = 127;
-      }
-    };
-    // one step: the next one's loads go out (into the other registers and the other buffer; past the end the last
-    // step's again, never used), then 4 x MI x TN MFMAs
-    auto step = [&](int buf, int s, uint4 (&qc)[TN], uint32_t (&sc)[TN], uint4 (&qo)[TN], uint32_t (&so)[TN]) {
-      arrive();
-      tail(buf, s);
-      load_a(buf ^ 1, min(s + 1, s1 - 1));
-      load_w(qo, so, min(s + 1, s1 - 1));
-      products(buf, [&](bf16x8_t (&b)[TN], int t) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) b[j] = mx4_cvt8(t == 0 ? qc[j].x : t == 1 ? qc[j].y : t == 2 ? qc[j].z : qc[j].w, mx4_scale(sc[j]));
-      });
     };
     if (s0 < s1) {
+      load_w(q, sw, s0);
       load_a(0, s0);
-      load_w(q, sb, s0);
     }
-    for (int s = s0; s < s1; s += 2) {
-      step(0, s, q, sb, qn, sbn);
-      if (s + 1 < s1) step(1, s + 1, qn, sbn, q, sb);
+    // One step: the next one's loads go out (past the end the last step's again, never used), then 4 x MI x TN MFMAs.
+    // This step's codes are claimed before them: the compiler waits for all loads in flight at the first use of one
+    // to a register while others go to LDS, and that wait has to fall where nothing newer is under way.
+    for (int s = s0; s < s1; ++s) {
+      const int buf = (s - s0) & 1;
+      arrive();
+#pragma unroll
+      for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(q[j].x), "+v"(q[j].y), "+v"(q[j].z), "+v"(q[j].w), "+v"(sw[j]));
+      tail(buf, s);
+      load_w(qn, swn, min(s + 1, s1 - 1));
+      load_a(buf ^ 1, min(s + 1, s1 - 1));
+      float sc[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sc[j] = mx4_scale(NARROW ? sw[j] : sw[j] >> ((s * 4 + kq - min(s * 4, ng - 4)) * 8 & 31) & 255u);
+      if (s * 4 + 4 > ng && s * 4 + kq >= ng) {  // lanes past the end of a row multiply zeros
+#pragma unroll
+        for (int j = 0; j < TN; ++j) q[j] = uint4{0, 0, 0, 0}, sc[j] = 1.f;
+      }
+      products(buf, [&](bf16x8_t (&b)[TN], int t) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) b[j] = mx4_cvt8(t == 0 ? q[j].x : t == 1 ? q[j].y : t == 2 ? q[j].z : q[j].w, sc[j]);
+      });
+#pragma unroll
+      for (int j = 0; j < TN; ++j) q[j] = qn[j], sw[j] = swn[j];
     }
   } else {
     constexpr int CLD = BN / 2 + 16;           // bytes of a staged code row: 16 rows of 8-B reads hit different banks
     constexpr int CBT = BN / 8;                // code bytes per thread: 8, 16 or 32
-    constexpr int NG = BN / 32, SPT = (64 * NG + 255) / 256;
+    constexpr int NG = BN / 32;                // scale groups of a code row: 2, 4 or 8; its four threads share them out
     char* cbase = smem + 2 * BM * 128;
     float* sbase = reinterpret_cast<float*>(cbase + 2 * 64 * CLD);
     const int crow = tid >> 2, cseg = (tid & 3) * CBT;
     const int ng = g.K / 32;
-    uint2 q[CBT / 8];
-    float sc[SPT];
+    uint2 q[CBT / 8];  // the next step's, on their way to LDS
+    uint32_t sw;
+    const int sgrp = NG == 8 ? (tid & 3) * 2 : (tid & 3) % NG;  // this thread's first group of the row
+    const int sfirst = NARROW ? c0 / 32 + sgrp : min(c0 / 32 + (sgrp & ~3), g.K / 32 - 4);
     auto load_c = [&](int s) {
-      const int n = s * 64 + crow;
-      const uint8_t* p = g.codes + (long)min(n, g.N - 1) * (g.K / 2) + c0 / 2 + cseg;
+      const uint8_t* p = g.codes + (long)min(s * 64 + crow, g.N - 1) * (g.K / 2);
 #pragma unroll
-      for (int e = 0; e < CBT / 8; ++e) {
-        q[e] = uint2{0, 0};
-        if (n < g.N && c0 + (cseg + e * 8) * 2 < g.K) q[e] = *reinterpret_cast<const uint2*>(p + e * 8);
-      }
-#pragma unroll
-      for (int e = 0; e < SPT; ++e) {
-        const int id = e * 256 + tid, sn = s * 64 + id / NG, gi = c0 / 32 + id % NG;
-        sc[e] = 1.f;
-        if (id < 64 * NG && sn < g.N && gi < ng) sc[e] = mx4_scale(g.scales[(long)sn * ng + gi]);
-      }
+      for (int e = 0; e < CBT / 8; ++e) q[e] = *reinterpret_cast<const uint2*>(p + min(c0 / 2 + cseg + e * 8, g.K / 2 - 8));
+      const uint8_t* sp = g.scales + (long)min(s * 64 + crow, g.N - 1) * ng;
+      if constexpr (NARROW) sw = sp[min(sfirst, ng - 1)];
+      else sw = load_u32(sp + sfirst);
     };
-    auto put_c = [&](int buf) {
+    // rows past N become zeros; columns past K are never stored
+    auto put_c = [&](int buf, int s) {
+      const bool in = s * 64 + crow < g.N;
+      char* cb = cbase + buf * 64 * CLD;
 #pragma unroll
-      for (int e = 0; e < CBT / 8; ++e) *reinterpret_cast<uint2*>(cbase + buf * 64 * CLD + crow * CLD + cseg + e * 8) = q[e];
+      for (int e = 0; e < CBT / 8; ++e) *reinterpret_cast<uint2*>(cb + crow * CLD + cseg + e * 8) = in ? q[e] : uint2{0, 0};
+      float* sb = sbase + buf * 64 * NG + crow;
 #pragma unroll
-      for (int e = 0; e < SPT; ++e) {
-        const int id = e * 256 + tid;
-        if (id < 64 * NG) sbase[buf * 64 * NG + (id % NG) * 64 + id / NG] = sc[e];
+      for (int e = 0; e < (NG == 8 ? 2 : 1); ++e) {
+        const uint32_t byte = NARROW ? sw : sw >> ((c0 / 32 + sgrp + e - sfirst) * 8 & 31) & 255u;
+        sb[(sgrp + e) * 64] = mx4_scale(in ? byte : 127u);
       }
     };
     if (s0 < s1) {
-      load_a(0, s0);
       load_c(s0);
-      put_c(0);
+      load_a(0, s0);
+      put_c(0, s0);
     }
     for (int s = s0; s < s1; ++s) {
       const int buf = (s - s0) & 1;
       arrive();
-      // the codes come out of LDS before the next step's loads start: the compiler would make a transposed read
-      // wait for every load to LDS in flight
+      // (before the next loads go out: the compiler makes a transposed read wait for every load to LDS in flight)
       i32x2_t raw[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
@@ -223,9 +237,10 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
           b[j] = mx4_cvt8((uint32_t)raw[j][h], *reinterpret_cast<const f32x4_t*>(p), *reinterpret_cast<const f32x4_t*>(p + 4));
         }
       });
-      put_c(buf ^ 1);
+      put_c(buf ^ 1, s + 1);
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
   // ---- store.  Lane: row i * 16 + r16, columns j * 16 + 4 kq + 0 .. 3; two column tiles are exchanged between
   // neighbouring lane groups so that a lane holds 8 columns in a row.
@@ -309,17 +324,50 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__
   for (int e = 0; e < V; ++e) y[m * ldy + c + e] = f2bf(v[e] + (bias ? bf2f(bias[c + e]) : 0.f));
 }
 
-template <int BM, int TN, bool DG, bool PART>
+// W^T in bf16: out[k, n] for n < N (N % 64 == 0), 64 rows of W x 256 columns per workgroup.  The codes go through LDS
+// and come back transposed, as in the dx tiles; a lane writes 16 values of one row of W^T, four lanes 128 B.
+__global__ __launch_bounds__(256) void mx4_dequant_t_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                            int N, int K, bf16_t* __restrict__ out) {
+  constexpr int CLD = 128 + 16;
+  __shared__ __attribute__((aligned(16))) char img[64 * CLD];
+  __shared__ __attribute__((aligned(16))) float sc[8 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r16 = lane & 15, kq = lane >> 4;
+  const int n0 = blockIdx.x * 64, c0 = blockIdx.y * 256, ng = K / 32;
+  const uint8_t* p = codes + (long)(n0 + (tid >> 2)) * (K / 2) + c0 / 2 + (tid & 3) * 32;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (c0 + (tid & 3) * 64 + e * 32 < K)
+      *reinterpret_cast<uint4*>(img + (tid >> 2) * CLD + (tid & 3) * 32 + e * 16) = *reinterpret_cast<const uint4*>(p + e * 16);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int id = e * 256 + tid, gi = c0 / 32 + (id & 7);
+    if (gi < ng) sc[(id & 7) * 64 + (id >> 3)] = mx4_scale(scales[(long)(n0 + (id >> 3)) * ng + gi]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const i32x2_t raw = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)(
+        img + lane * CLD + (w * 4 + j) * 8));
+    const float* s = sc + ((w * 4 + j) >> 1) * 64 + kq * 16;
+    const int k = c0 + (w * 4 + j) * 16 + r16;
+    if (k >= K) continue;
+    bf16x8_t* o = reinterpret_cast<bf16x8_t*>(out + (long)k * N + n0 + kq * 16);
+    o[0] = mx4_cvt8((uint32_t)raw[0], *reinterpret_cast<const f32x4_t*>(s), *reinterpret_cast<const f32x4_t*>(s + 4));
+    o[1] = mx4_cvt8((uint32_t)raw[1], *reinterpret_cast<const f32x4_t*>(s + 8), *reinterpret_cast<const f32x4_t*>(s + 12));
+  }
+}
+
+template <int BM, int TN, bool DG, bool PART, bool NARROW = false>
 void launch_k(const Mx4LinearArgs& a, const Mx4Plan& p, hipStream_t st) {
   constexpr int shm = lds_bytes<BM, TN, DG>();
   static const bool once = [] {
-    MFT_HIP_CHECK(hipFuncSetAttribute((const void*)mx4_tile_kernel<BM, TN, DG, PART>, hipFuncAttributeMaxDynamicSharedMemorySize, shm));
+    MFT_HIP_CHECK(hipFuncSetAttribute((const void*)mx4_tile_kernel<BM, TN, DG, PART, NARROW>, hipFuncAttributeMaxDynamicSharedMemorySize, shm));
     return true;
   }();
   (void)once;
   const int cols = DG ? a.K : a.N;
   const long tiles = (long)((a.M + BM - 1) / BM) * ((cols + 64 * TN - 1) / (64 * TN)) * p.splits;
-  mx4_tile_kernel<BM, TN, DG, PART><<<(unsigned)tiles, 256, shm, st>>>(a, p.splits);
+  mx4_tile_kernel<BM, TN, DG, PART, NARROW><<<(unsigned)tiles, 256, shm, st>>>(a, p.splits);
 }
 
 template <int BM, int TN>
@@ -339,6 +387,7 @@ Mx4Plan mx4_plan(int M, int N, int K, bool dgrad) {
   Mx4Plan p{};
   p.bm = 128, p.tn = 4, p.splits = 1;
   if (const char* e = getenv("MX4_PLAN")) sscanf(e, "%d,%d,%d", &p.bm, &p.tn, &p.splits);
+  if (K < 128) p.bm = 64, p.tn = 2, p.splits = dgrad ? p.splits : 1;
   return p;
 }
 
@@ -346,8 +395,34 @@ long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad) {
   return p.splits > 1 ? (long)p.splits * M * (dgrad ? K : N) : 0;
 }
 
+bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx) {
+  return ldx % 8 == 0 && (dgrad ? gemm4_supported(M, K, N, false, false) && K % 8 == 0 : gemm4_supported(M, N, K, false, false));
+}
+
+void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st) {
+  GemmArgs f{};
+  f.A = a.x; f.lda = a.ldx;
+  f.B = w;
+  f.C = a.y; f.ldc = a.ldy;
+  f.M = a.M; f.alpha = 1.f;
+  if (dgrad) {
+    mx4_dequant_t_kernel<<<dim3(a.N / 64, (a.K + 255) / 256), 256, 0, st>>>(a.codes, a.scales, a.N, a.K, w);
+    f.ldb = a.N; f.N = a.K; f.K = a.N;
+    gemm4x(f, GEMM_EPI_NONE, false, false, st);
+  } else {
+    mx4_dequantize(a.codes, a.scales, 0, a.N, a.K, w, a.K, a.N, a.K, st);
+    f.ldb = a.K; f.N = a.N; f.K = a.K;
+    f.bias = a.bias;
+    gemm4x(f, a.bias ? GEMM_EPI_BIAS : GEMM_EPI_NONE, false, false, st);
+  }
+}
+
 void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st) {
-  if (p.bm == 128 && p.tn == 4) launch<128, 4>(a, p, dgrad, st);
+  if (a.K < 128) {
+    if (dgrad && p.splits > 1) launch_k<64, 2, true, true, true>(a, p, st);
+    else if (dgrad) launch_k<64, 2, true, false, true>(a, p, st);
+    else launch_k<64, 2, false, false, true>(a, p, st);
+  } else if (p.bm == 128 && p.tn == 4) launch<128, 4>(a, p, dgrad, st);
   else if (p.bm == 128 && p.tn == 2) launch<128, 2>(a, p, dgrad, st);
   else if (p.bm == 64 && p.tn == 4) launch<64, 4>(a, p, dgrad, st);
   else if (p.bm == 64 && p.tn == 2) launch<64, 2>(a, p, dgrad, st);

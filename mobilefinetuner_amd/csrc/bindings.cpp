@@ -416,17 +416,17 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   a.bias = optp<bf16_t>(bias);
   a.y = bp(y); a.ldy = out;
   a.M = (int)x2.size(0); a.N = (int)N; a.K = K;
-  if (!dgrad && a.M <= 64 && !(getenv("MX4_ROWS") && getenv("MX4_ROWS")[0] == 48)) {
+  if (!dgrad && mft::mx4_few_rows(a.M, a.N, a.K)) {
     mft::mx4_rows(a, stream());
     return y;
   }
-  if (getenv("MX4_DENSE") && getenv("MX4_DENSE")[0] == '1' && mft::mx4_dense_supported(a.M, a.N, a.K, dgrad, a.ldx)) {
-    const Tensor w = torch::empty({N * K}, x.options());
-    mft::mx4_dense(a, bp(w), dgrad, stream());
+  const auto plan = mft::mx4_plan(a.M, a.N, a.K, dgrad, a.ldx);
+  Tensor ws;
+  if (plan.dense) {
+    ws = torch::empty({N * K}, x.options());
+    mft::mx4_dense(a, bp(ws), dgrad, stream());
     return y;
   }
-  const auto plan = mft::mx4_plan(a.M, a.N, a.K, dgrad);
-  Tensor ws;
   if (const long n = mft::mx4_plan_ws_floats(plan, a.M, a.N, a.K, dgrad)) {
     ws = torch::empty({n}, x.options().dtype(torch::kFloat32));
     a.ws = fp(ws);

@@ -403,14 +403,18 @@ struct Mx4LinearArgs {
   int M, N, K;
   float* ws;  // mx4_plan_ws_floats
 };
-void mx4_rows(const Mx4LinearArgs& a, hipStream_t st);  // y = x W^T + bias, M <= 64 (mx4.hip)
+// y = x W^T + bias for few rows (mx4.hip): mx4_few_rows says whether (non-zero) it is the kernel for a product
+int mx4_few_rows(int M, int N, int K);
+void mx4_rows(const Mx4LinearArgs& a, hipStream_t st);
+// y, or dx = dy W, by tiles that convert the weight in registers, or (dense) through a bf16 copy of W (of W^T for dx,
+// N * K elements) and gemm4 (mx4_gemm.hip).  The plan goes by the sizes alone.
 struct Mx4Plan {
   int bm, tn, splits;  // rows and 64-column strips of a tile, workgroups that share a tile's reduction
+  int dense;
 };
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad);
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx);
 long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad);
-void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);  // y, or dx = dy W (mx4_gemm.hip)
-// the same through a bf16 copy of W (W^T for dx) in w [N * K] and gemm4
+void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);
 bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx);
 void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st);
 

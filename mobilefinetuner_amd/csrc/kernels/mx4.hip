@@ -208,6 +208,112 @@ __global__ __launch_bounds__(64 * (S > 4 ? S : 4)) void mx4_rows_kernel(Mx4Linea
     }
 }
 
+// ------------------------------------------------------------------ y = x W^T + b, up to 16 rows, many columns
+// Streams the codes once: a wave owns 32 columns and walks K in steps of 256, a lane reading 32 B of its row (two
+// scale groups: columns 256 s + 64 (l >> 4) .. + 63), so a step takes whole 128-B lines.  x sits in LDS, read with
+// the same permutation; rows M .. 15 of the operand repeat row M - 1 and are never stored.  No barrier in the loop.
+// 4 x 262144 x 1152: 37.5 us (4.4 TB/s of codes; the same through the tiles of mx4_gemm 43 us, through mx4_rows 45 us).
+// Measured and not kept: waves that go on to further strips with x already in LDS (38.4 us), 8 waves per SIMD (spills).
+__global__ __launch_bounds__(256) void mx4_stream_kernel(Mx4LinearArgs g) {
+  extern __shared__ __attribute__((aligned(16))) bf16_t xs[];
+  constexpr int TN = 2;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = lane >> 4;
+  const int ng = g.K / 32, kb = g.K / 2, ldxs = g.K + 8;
+  const int n0 = blockIdx.x * (64 * TN) + w * (16 * TN);
+  const uint8_t* cb = g.codes + (long)n0 * kb;
+  const uint8_t* sb = g.scales + (long)n0 * ng;
+  uint32_t co[TN], so[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = min(j * 16 + r16, max(g.N - 1 - n0, 0));
+    co[j] = (uint32_t)(n * kb), so[j] = (uint32_t)(n * ng);
+  }
+  const bool live = n0 < g.N;  // (a wave past the last column only helps to fetch x)
+  if (!live) cb = g.codes, sb = g.scales;
+  struct Step {
+    uint4 q[TN][2];
+    uint32_t sw[TN];
+  };
+  auto load = [&](Step& t, int s) {
+    const int g0 = s * 8 + kq * 2, c0 = min(g0, ng - 1) * 16, c1 = min(g0 + 1, ng - 1) * 16, gs = min(g0, ng - 4);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      t.q[j][0] = *reinterpret_cast<const uint4*>(cb + (co[j] + c0));
+      t.q[j][1] = *reinterpret_cast<const uint4*>(cb + (co[j] + c1));
+      __builtin_memcpy(&t.sw[j], sb + (so[j] + gs), 4);
+    }
+  };
+  const int steps = (ng + 7) / 8;
+  Step a, b;
+  load(a, 0);
+  {
+    const int k8 = g.K / 8, n = g.M * k8;
+    for (int i = tid; i < n; i += 256) {
+      const int r = i / k8, c = i - r * k8;
+      *reinterpret_cast<uint4*>(xs + r * ldxs + c * 8) = *reinterpret_cast<const uint4*>(g.x + (long)r * g.ldx + c * 8);
+    }
+  }
+  __syncthreads();
+  if (!live) return;
+  const bf16_t* xr = xs + min(r16, g.M - 1) * ldxs;
+  f32x4_t acc[TN] = {zero4(), zero4()};
+  auto use = [&](Step& t, int s) {
+    const int g0 = s * 8 + kq * 2, sh = (g0 - min(g0, ng - 4)) * 8;
+    float sc[TN][2];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sc[j][0] = mx4_scale(t.sw[j] >> (sh & 31) & 255u), sc[j][1] = mx4_scale(t.sw[j] >> (sh + 8 & 31) & 255u);
+    if (s * 8 + 8 > ng) {  // groups past the end of the row multiply zeros (their x reads repeat the last group)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (g0 + e >= ng)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) t.q[j][e] = uint4{0, 0, 0, 0}, sc[j][e] = 1.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool in = s * 8 + 8 <= ng || g0 + e < ng;
+      const bf16_t* xp = xr + min(g0 + e, ng - 1) * 32;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        bf16x8_t xv = *reinterpret_cast<const bf16x8_t*>(xp + u * 8);
+        if (!in) xv = bf16x8_t{};
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const uint32_t c = u == 0 ? t.q[j][e].x : u == 1 ? t.q[j][e].y : u == 2 ? t.q[j][e].z : t.q[j][e].w;
+          acc[j] = mfma16(mx4_cvt8(c, sc[j][e]), xv, acc[j]);
+        }
+      }
+    }
+  };
+  int s = 0;
+  for (; s + 1 < steps; s += 2) {
+    load(b, s + 1);
+    use(a, s);
+    load(a, min(s + 2, steps - 1));
+    use(b, s + 1);
+  }
+  if (s < steps) use(a, s);
+  if (r16 >= g.M) return;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int nc = n0 + j * 16 + 4 * kq;
+    if (nc >= g.N) continue;
+    bf16_t* y = g.y + (long)r16 * g.ldy + nc;
+    f32x4_t v = acc[j];
+    if (nc + 4 <= g.N && g.ldy % 4 == 0) {
+      if (g.bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += bf2f(g.bias[nc + r]);
+      }
+      *reinterpret_cast<uint2*>(y) = uint2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (nc + r < g.N) y[r] = f2bf(v[r] + (g.bias ? bf2f(g.bias[nc + r]) : 0.f));
+    }
+  }
+}
+
 void check_grid(long blocks, const char* what) {
   if (blocks > 0x7fffffffL) {
     fprintf(stderr, "mft::%s: %ld workgroups exceed a grid\n", what, blocks);
@@ -249,17 +355,14 @@ static void launch_rows(const Mx4LinearArgs& a, hipStream_t st) {
   mx4_rows_kernel<MT, TN, S, U><<<(a.N + per - 1) / per, 64 * (S > 4 ? S : 4), 0, st>>>(a);
 }
 
-// waves that split K, from the waves that the column tiles alone give
+// S: the waves that share a column tile, until tiles x S fill the SIMDs (each 1/S of K is at least one chunk)
 template <int MT>
 static void launch_rows_mt(const Mx4LinearArgs& a, hipStream_t st) {
   const int tiles = (a.N + 15) / 16, chunks = (a.K + 127) / 128;
-  const int force = getenv("MX4_S") ? atoi(getenv("MX4_S")) : 0;
-  int S = 1;
-  while (S < 16 && S < chunks && (long)tiles * S < 4096) S *= 2;
-  if (force) S = force;
+  int S = 2;
+  while (S < 16 && S < chunks && (long)tiles * S < 2048) S *= 2;
   constexpr int U = MT == 1 ? 2 : 1;
   switch (S) {
-    case 1: launch_rows<MT, 2, 1, U>(a, st); break;
     case 2: launch_rows<MT, 1, 2, U>(a, st); break;
     case 4: launch_rows<MT, 1, 4, U>(a, st); break;
     case 8: launch_rows<MT, 1, 8, U>(a, st); break;
@@ -267,7 +370,24 @@ static void launch_rows_mt(const Mx4LinearArgs& a, hipStream_t st) {
   }
 }
 
+// The kernel of a forward product of few rows: 1 mx4_rows, 2 mx4_stream, 0 the tiles of mx4_gemm.hip.  Measured (us,
+// rows / stream / best tile): 1 x 2304 x 768 3.5 / 4.6 / 4.7; 4 x 13824 x 1152 7.6 / 6.2 / 7.4; 16 x 6400 x 1600 9.7 / 9.0 / 8.8;
+// 16 x 1152 x 6912 12.4 / - / 9.8; 24 x 768 x 2304 7.2 / - / 8.5; 64 x 2304 x 768 6.4 / - / 7.0; 64 x 768 x 2304 12 / - / 8.9;
+// 64 x 13824 x 1152 21.9 / - / 11.9.  The stream wins once its 128-column strips fill a good part of the chip; mx4_rows
+// reads x once per column tile and loses when that is much, by length or by the number of tiles.
+int mx4_few_rows(int M, int N, int K) {
+  if (M > 64) return 0;
+  if (M <= 16 && N >= 12800 && K >= 128 && (long)M * (K + 8) * 2 <= 65536) return 2;
+  const int mt = (M + 15) / 16;
+  if (mt == 1) return N < 12800 && M * K <= 80000 ? 1 : 0;
+  return mt * K <= 5000 && N <= 8192 ? 1 : 0;
+}
+
 void mx4_rows(const Mx4LinearArgs& a, hipStream_t st) {
+  if (mx4_few_rows(a.M, a.N, a.K) == 2) {
+    mx4_stream_kernel<<<(a.N + 127) / 128, 256, (size_t)a.M * (a.K + 8) * 2, st>>>(a);
+    return;
+  }
   if (a.M <= 16) launch_rows_mt<1>(a, st);
   else if (a.M <= 32) launch_rows_mt<2>(a, st);
   else if (a.M <= 48) launch_rows_mt<3>(a, st);

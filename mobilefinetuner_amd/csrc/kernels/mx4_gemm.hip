@@ -15,6 +15,7 @@
 #include "mx4.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <type_traits>
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
   // T sub-steps of 32 reduction columns, each MI x TN MFMAs, in blocks of HB row tiles: while a block multiplies, the
   // next one's activation operands are read, and in a sub-step's last block the next sub-step's weight operands are
   // converted (conv(b, t)).  The scheduling barriers keep the compiler from pulling each read down to its first use.
-  constexpr int HB = MI < 4 || (!DG && MI * TN == 32) ? 2 : 4, T = STEP / 32, NB = T * MI / HB;  // (128 x 256: 4 would spill)
+  constexpr int HB = MI == 1 ? 1 : MI < 4 || (!DG && MI * TN == 32) ? 2 : 4, T = STEP / 32, NB = T * MI / HB;  // (128 x 256: 4 would spill)
   auto frag_a = [&](int buf, int i, int t) {
     const int row = i * 16 + r16;
     return *reinterpret_cast<const bf16x8_t*>(abuf(buf) + (row * CPR + ((t * 4 + kq) ^ swz(row))) * 8);
@@ -383,12 +384,54 @@ void launch(const Mx4LinearArgs& a, const Mx4Plan& p, bool dg, hipStream_t st) {
 
 }  // namespace
 
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad) {
-  Mx4Plan p{};
-  p.bm = 128, p.tn = 4, p.splits = 1;
-  if (const char* e = getenv("MX4_PLAN")) sscanf(e, "%d,%d,%d", &p.bm, &p.tn, &p.splits);
-  if (K < 128) p.bm = 64, p.tn = 2, p.splits = dgrad ? p.splits : 1;
-  return p;
+namespace {
+
+// Modelled time of a tile shape, in us: a0 + steps of a workgroup x max(lat, workgroups per CU x thr) + workgroups per
+// CU x fix (+ the join: j0 + slab bytes at jb TB/s).  lat: a step alone on its CU, bound by a load's latency; thr: a step's
+// share of a busy CU; fix: a workgroup's start and stores.  Fitted to 320 products (1 to 16,384 rows, 12 weights, every
+// shape and split): the shape picked costs 3 % (y) and 6 % (dx) over the best one on average, at worst 22 % and 42 %.
+struct TileCost {
+  int bm, tn;
+  float lat, thr, fix;
+};
+constexpr TileCost kCostY[] = {{128, 4, 2.07f, 1.32f, 4.4f}, {128, 2, 1.27f, 0.86f, 2.5f}, {64, 4, 1.37f, 0.90f, 2.8f},
+                               {64, 2, 0.87f, 0.55f, 1.7f},  {64, 1, 0.64f, 0.43f, 1.2f},  {32, 2, 0.66f, 0.41f, 1.3f},
+                               {32, 1, 0.47f, 0.30f, 0.85f}, {16, 1, 0.45f, 0.26f, 0.8f}};
+constexpr TileCost kCostDx[] = {{128, 4, 1.28f, 0.78f, 3.5f}, {128, 2, 0.81f, 0.48f, 1.9f}, {64, 4, 0.96f, 0.54f, 1.9f},
+                                {64, 2, 0.66f, 0.36f, 1.2f},  {64, 1, 0.55f, 0.29f, 0.78f}, {32, 2, 0.56f, 0.30f, 0.81f},
+                                {32, 1, 0.49f, 0.20f, 0.61f}};
+
+}  // namespace
+
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx) {
+  if (K < 128) return Mx4Plan{64, 2, 1, 0};  // the narrow kernel
+  const long cols = dgrad ? K : N, red = dgrad ? N : K;
+  const long steps = dgrad ? (red + 63) / 64 : (red + 127) / 128;
+  Mx4Plan best{};
+  double best_t = 1e30;
+  auto consider = [&](const TileCost& c) {
+    if (M <= c.bm / 2 && c.bm > 32) return;  // (32 rows: the smallest dx tile)
+    const long tiles = (M + c.bm - 1L) / c.bm * ((cols + 64 * c.tn - 1) / (64 * c.tn));
+    for (int s = 1; s <= 32; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : 8) {
+      if (s > 1 && (steps / s < 2 || tiles * s > 2048)) break;
+      const double n = (double)((tiles * s + 255) / 256), per = (double)((steps + s - 1) / s);
+      double t = (dgrad ? 2.6 : 3.0) + per * std::max((double)c.lat, n * c.thr) + n * c.fix;
+      if (s > 1) t += (dgrad ? 4.2 : 3.2) + (double)s * M * cols * 4 / 3.2e6;
+      if (t < best_t) best_t = t, best = Mx4Plan{c.bm, c.tn, s, 0};
+    }
+  };
+  if (dgrad)
+    for (const TileCost& c : kCostDx) consider(c);
+  else
+    for (const TileCost& c : kCostY) consider(c);
+  // through a bf16 copy: its writing and reading at 4.5 TB/s, then 256 x 256 tiles of gemm4 in K steps of 64 -- 1.15 us alone
+  // on a CU, 1.5 us when every CU is busy -- and about 4 us per round of tiles
+  if (mx4_dense_supported(M, N, K, dgrad, ldx)) {
+    const double tiles = (double)((M + 255L) / 256 * ((cols + 255) / 256)), rounds = std::ceil(tiles / 256), st = red / 64.0;
+    const double t = 5 + (double)N * K * 2.53 / 4.5e6 + std::max(rounds * (st * 1.15 + 4), tiles / 256 * (st * 1.5 + 1));
+    if (t < best_t) best = Mx4Plan{0, 0, 1, 1};
+  }
+  return best;
 }
 
 long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad) {
@@ -418,17 +461,19 @@ void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st) {
 }
 
 void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st) {
+  const int shape = p.bm * 10 + p.tn;
   if (a.K < 128) {
-    if (dgrad && p.splits > 1) launch_k<64, 2, true, true, true>(a, p, st);
-    else if (dgrad) launch_k<64, 2, true, false, true>(a, p, st);
+    if (dgrad) launch_k<64, 2, true, false, true>(a, p, st);
     else launch_k<64, 2, false, false, true>(a, p, st);
-  } else if (p.bm == 128 && p.tn == 4) launch<128, 4>(a, p, dgrad, st);
-  else if (p.bm == 128 && p.tn == 2) launch<128, 2>(a, p, dgrad, st);
-  else if (p.bm == 64 && p.tn == 4) launch<64, 4>(a, p, dgrad, st);
-  else if (p.bm == 64 && p.tn == 2) launch<64, 2>(a, p, dgrad, st);
-  else if (p.bm == 64 && p.tn == 1) launch<64, 1>(a, p, dgrad, st);
-  else if (p.bm == 32 && p.tn == 2) launch<32, 2>(a, p, dgrad, st);
-  else if (p.bm == 32 && p.tn == 1) launch<32, 1>(a, p, dgrad, st);
+  } else if (shape == 1284) launch<128, 4>(a, p, dgrad, st);
+  else if (shape == 1282) launch<128, 2>(a, p, dgrad, st);
+  else if (shape == 644) launch<64, 4>(a, p, dgrad, st);
+  else if (shape == 642) launch<64, 2>(a, p, dgrad, st);
+  else if (shape == 641) launch<64, 1>(a, p, dgrad, st);
+  else if (shape == 322) launch<32, 2>(a, p, dgrad, st);
+  else if (shape == 321) launch<32, 1>(a, p, dgrad, st);
+  else if (shape == 161 && !dgrad && p.splits > 1) launch_k<16, 1, false, true>(a, p, st);
+  else if (shape == 161 && !dgrad) launch_k<16, 1, false, false>(a, p, st);
   else {
     fprintf(stderr, "mft::mx4_tiles: no kernel for tile %d x %d\n", p.bm, 64 * p.tn);
     abort();

@@ -29,18 +29,18 @@ __device__ __forceinline__ long ratio_pos(int R) {
   return (R & ~255) + (rl >> 6) * 64 + (rl & 15) * 4 + ((rl >> 4) & 3);
 }
 
-// One workgroup: the valid rows counted, w = 1 / max(1, count), the running state cleared, the labels of the
-// first piece (relative to it, -100 elsewhere).
+// The running state cleared, the labels of the first piece (relative to it, -100 elsewhere), and the valid rows
+// counted per workgroup (count_valid sums the counts: whole numbers, any order).
 __global__ __launch_bounds__(1024) void ce_pieces_begin_kernel(const int64_t* __restrict__ labels, int M, int V, int w0,
                                                                int64_t* __restrict__ rel, float* __restrict__ run_m,
                                                                float* __restrict__ run_s, float* __restrict__ lbl,
-                                                               float* __restrict__ zero, float* __restrict__ weight,
-                                                               int64_t* __restrict__ n_valid) {
+                                                               float* __restrict__ zero, float* __restrict__ counts) {
   __shared__ float red[16];
-  float n = 0.f;  // M < 2^24: exact in fp32
-  for (int i = threadIdx.x; i < M; i += 1024) {
+  const int i = blockIdx.x * 1024 + threadIdx.x;
+  float n = 0.f;
+  if (i < M) {
     const int64_t l = labels[i];
-    if (l >= 0 && l < V) n += 1.f;
+    if (l >= 0 && l < V) n = 1.f;
     rel[i] = l >= 0 && l < w0 ? l : -100;
     run_m[i] = -INFINITY;
     run_s[i] = 0.f;
@@ -48,10 +48,14 @@ __global__ __launch_bounds__(1024) void ce_pieces_begin_kernel(const int64_t* __
     zero[i] = 0.f;
   }
   n = block_sum(n, red);
-  if (threadIdx.x == 0) {
-    *weight = 1.f / fmaxf(n, 1.f);
-    *n_valid = (int64_t)n;
-  }
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// by a whole wave; M <= 2^24, so the sum is exact in fp32
+__device__ __forceinline__ float count_valid(const float* counts, int M) {
+  float n = 0.f;
+  for (int i = threadIdx.x & 63; i < (M + 1023) / 1024; i += 64) n += counts[i];
+  return wave_sum(n);
 }
 
 // RB rows per block.  Pass 1 (a wave per row, lanes over the piece's tiles): the piece's maximum and sum join the
@@ -128,23 +132,54 @@ __global__ __launch_bounds__(256) void ce_piece_merge_kernel(const float* __rest
   *reinterpret_cast<f32x4_t*>(acc + i) = a;
 }
 
-// a wave per row: its loss and, with dh, its gradient
+// WPR waves per row: its loss and, with dh, its gradient.  The last piece's sum comes in here: S > 0 slabs of a split
+// product (on top of acc * accscale when there were pieces before it), or acc alone.  WPR = 4 (few rows): the waves share
+// the slabs out and wave 0 adds their four sums in order (512 rows, 40 slabs: 29 us by one wave per row).
+template <int WPR>
 __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __restrict__ run_m, const float* __restrict__ run_s,
                                                              const float* __restrict__ lbl, const int64_t* __restrict__ labels,
-                                                             int M, int K, int V, const float* __restrict__ weight,
-                                                             const float* __restrict__ acc, const bf16_t* __restrict__ W,
-                                                             long ldw, const uint8_t* __restrict__ codes,
+                                                             int M, int K, int V, const float* __restrict__ counts,
+                                                             const float* __restrict__ acc, const float* __restrict__ accscale,
+                                                             const float* __restrict__ slab, int S,
+                                                             const bf16_t* __restrict__ W, long ldw,
+                                                             const uint8_t* __restrict__ codes,
                                                              const uint8_t* __restrict__ scales, float* __restrict__ loss_rows,
                                                              bf16_t* __restrict__ dh) {
-  const int R = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  __shared__ f32x4_t part[WPR > 1 ? 3 * 128 : 1];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int R = WPR > 1 ? blockIdx.x : blockIdx.x * 4 + w, ws = WPR > 1 ? w : 0;
   if (R >= M) return;
   const int64_t lab = labels[R];
   const bool valid = lab >= 0 && lab < V;
   const float s = run_s[R], lse = run_m[R] + __logf(s), nll = lse - lbl[R];
-  if (lane == 0) loss_rows[R] = valid ? nll : 0.f;
+  if (lane == 0 && ws == 0) loss_rows[R] = valid ? nll : 0.f;
   if (!dh) return;
-  const float wt = *weight, fa = wt / s, fl = wt * -expm1f(-nll);  // 1 - p = 1 - exp(l - lse)
-  for (int c = lane * 8; c < K; c += 512) {
+  const float wt = 1.f / fmaxf(count_valid(counts, M), 1.f), fa = wt / s, fl = wt * -expm1f(-nll);  // 1 - p = 1 - exp(l - lse)
+  const float old = accscale ? accscale[R] : 1.f;
+  for (int c0 = 0; c0 < K; c0 += 512) {
+    const int c = c0 + lane * 8;
+    f32x4_t a = zero4(), b = zero4();
+    if (c < K && valid) {
+#pragma unroll 4
+      for (int sp = ws; sp < S; sp += WPR) {
+        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(slab + ((long)sp * M + R) * K + c);
+        a += p[0];
+        b += p[1];
+      }
+      if (acc && ws == 0) {
+        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(acc + (long)R * K + c);
+        a += p[0] * old;
+        b += p[1] * old;
+      }
+    }
+    if constexpr (WPR > 1) {
+      __syncthreads();
+      if (ws) part[(ws - 1) * 128 + lane * 2] = a, part[(ws - 1) * 128 + lane * 2 + 1] = b;
+      __syncthreads();
+      if (ws) continue;
+      for (int i = 0; i < 3; ++i) a += part[i * 128 + lane * 2], b += part[i * 128 + lane * 2 + 1];
+    }
+    if (c >= K) continue;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (valid) {
       float wl[8];
@@ -154,22 +189,29 @@ __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __rest
 #pragma unroll
         for (int j = 0; j < 8; ++j) wl[j] = (float)v[j];
       }
-      const float* a = acc + (long)R * K + c;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = a[j] * fa - wl[j] * fl;
+      for (int j = 0; j < 4; ++j) {
+        o[j] = a[j] * fa - wl[j] * fl;
+        o[4 + j] = b[j] * fa - wl[4 + j] * fl;
+      }
     }
     store8(dh + (long)R * K + c, o);
   }
 }
 
-// one workgroup, fixed order: loss = weight * sum of the rows' losses
+// one workgroup, fixed order: loss = sum of the rows' losses / valid rows
 __global__ __launch_bounds__(1024) void ce_pieces_loss_kernel(const float* __restrict__ loss_rows, int M,
-                                                              const float* __restrict__ weight, float* __restrict__ loss) {
+                                                              const float* __restrict__ counts, float* __restrict__ loss,
+                                                              int64_t* __restrict__ n_valid) {
   __shared__ float red[16];
   float s = 0.f;
   for (int i = threadIdx.x; i < M; i += 1024) s += loss_rows[i];
   s = block_sum(s, red);
-  if (threadIdx.x == 0) *loss = s * *weight;
+  const float n = count_valid(counts, M);
+  if (threadIdx.x == 0) {
+    *loss = s / fmaxf(n, 1.f);
+    *n_valid = (int64_t)n;
+  }
 }
 
 // rows of the operand copied with zero padding: out [rows, kpad], in [rows_in >= .., K] (ragged last piece)
@@ -196,7 +238,7 @@ int num_cus() {
 }
 
 struct Layout {
-  float *run_m, *run_s, *lbl, *zero, *accscale, *weight, *stats, *ratio, *fin, *slab, *acc;
+  float *run_m, *run_s, *lbl, *zero, *accscale, *counts, *stats, *ratio, *fin, *slab, *acc;
   int64_t* rel;
   bf16_t *E, *wb;
   long bytes;
@@ -237,7 +279,7 @@ Layout make_layout(const CePiecesArgs& a, const Plan& p) {
   };
   auto floats = [&](long n) { return reinterpret_cast<float*>(take(n * 4)); };
   L.run_m = floats(M), L.run_s = floats(M), L.lbl = floats(M), L.zero = floats(M), L.accscale = floats(M);
-  L.weight = floats(1);
+  L.counts = floats((M + 1023) / 1024);
   L.rel = reinterpret_cast<int64_t*>(take(M * 8));
   L.stats = floats(2 * M * T);
   if (a.dh) {
@@ -255,8 +297,9 @@ Layout make_layout(const CePiecesArgs& a, const Plan& p) {
 }  // namespace
 
 int lm_head_ce_pieces_width(long M, int V) {
-  // E [M, piece] bf16 of 512 MiB, at least 4,096 columns (fewer launches and longer reductions per piece)
-  const long w = (512L << 20) / (2 * std::max(M, 1L)) / 256 * 256;
+  // E [M, piece] bf16 of 2 GiB, at least 4,096 columns.  16384 x 262144 x 640 in ms by columns of a piece: 4,096 17.4,
+  // 16,384 (512 MiB) 12.6, 65,536 (2 GiB) 11.5, the whole vocabulary (8 GiB) 11.5.
+  const long w = (2L << 30) / (2 * std::max(M, 1L)) / 256 * 256;
   return (int)std::min(std::max(w, 4096L), (long)(V + 255) / 256 * 256);
 }
 
@@ -272,10 +315,12 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
   const Layout L = make_layout(a, p);
   const long mpad = (long)((a.M + 255) / 256) * 256;
   const bool grad = a.dh != nullptr;
-  ce_pieces_begin_kernel<<<1, 1024, 0, st>>>(a.labels, a.M, a.V, p.n > 1 ? p.width : p.last, L.rel, L.run_m, L.run_s, L.lbl,
-                                             L.zero, L.weight, a.n_valid);
+  ce_pieces_begin_kernel<<<(a.M + 1023) / 1024, 1024, 0, st>>>(a.labels, a.M, a.V, p.n > 1 ? p.width : p.last, L.rel, L.run_m,
+                                                               L.run_s, L.lbl, L.zero, L.counts);
+  // rows per workgroup of the finalize: fewer while the workgroups do not fill the chip twice
   int rb = 64;
-  for (; rb > 16 && (a.M + rb - 1) / rb < 2 * num_cus(); rb /= 2) {}
+  for (; rb > 4 && (a.M + rb - 1) / rb < 2 * num_cus(); rb /= 2) {}
+  int last_slabs = 0;
   for (int i = 0; i < p.n; ++i) {
     const int v0 = i * p.width, w = i + 1 < p.n ? p.width : p.last, wp = up64(w), T = (wp + 255) / 256;
     const bf16_t* W = a.W ? a.W + (long)v0 * a.ldw : nullptr;
@@ -300,7 +345,11 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
     else gemm8x(f, GEMM_EPI_CE_FWD, false, false, st);
     const int S = grad ? ce_dgrad_splits(a.M, a.K, wp) : 1;
     const int tps = S > 1 ? ((wp / 64 + S - 1) / S) / 4 : T;
-    auto fk = rb == 64 ? ce_piece_finalize_kernel<64> : rb == 32 ? ce_piece_finalize_kernel<32> : ce_piece_finalize_kernel<16>;
+    auto fk = rb == 64   ? ce_piece_finalize_kernel<64>
+              : rb == 32 ? ce_piece_finalize_kernel<32>
+              : rb == 16 ? ce_piece_finalize_kernel<16>
+              : rb == 8  ? ce_piece_finalize_kernel<8>
+                         : ce_piece_finalize_kernel<4>;
     const int next0 = v0 + w, next_w = i + 1 >= p.n ? 0 : i + 2 < p.n ? p.width : p.last;
     fk<<<(a.M + rb - 1) / rb, 256, 0, st>>>(reinterpret_cast<const float2*>(L.stats), a.M, T, mpad, a.labels, next0, next_w,
                                             L.rel, L.run_m, L.run_s, grad ? L.accscale : nullptr, grad ? L.E : nullptr, wp,
@@ -315,6 +364,10 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
       d.ksplit = S;
       d.ws = L.slab;
       gemm8x(d, GEMM_EPI_CE_DGRAD, false, true, st);
+      if (i + 1 == p.n) {
+        last_slabs = S;
+        break;
+      }
       const long n4 = (long)a.M * a.K / 4;
       ce_piece_merge_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(L.slab, S, a.M, a.K, i ? L.accscale : nullptr, L.acc);
     } else {
@@ -323,9 +376,11 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
       gemm8x(d, GEMM_EPI_CE_DGRAD_ACC, false, true, st);
     }
   }
-  ce_pieces_rows_kernel<<<(a.M + 3) / 4, 256, 0, st>>>(L.run_m, L.run_s, L.lbl, a.labels, a.M, a.K, a.V, L.weight, L.acc, a.W,
-                                                       a.ldw, a.codes, a.scales, a.loss_rows, a.dh);
-  ce_pieces_loss_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.M, L.weight, a.loss);
+  auto rk = last_slabs >= 8 ? ce_pieces_rows_kernel<4> : ce_pieces_rows_kernel<1>;
+  rk<<<last_slabs >= 8 ? a.M : (a.M + 3) / 4, 256, 0, st>>>(
+      L.run_m, L.run_s, L.lbl, a.labels, a.M, a.K, a.V, L.counts, last_slabs && p.n == 1 ? nullptr : L.acc,
+      last_slabs ? L.accscale : nullptr, L.slab, last_slabs, a.W, a.ldw, a.codes, a.scales, a.loss_rows, a.dh);
+  ce_pieces_loss_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.M, L.counts, a.loss, a.n_valid);
 }
 
 }  // namespace mft

@@ -402,6 +402,7 @@ struct Mx4LinearArgs {
   long ldy;
   int M, N, K;
   float* ws;  // mx4_plan_ws_floats
+  int slabs_only;  // mx4_tiles, K >= 128: leave the fp32 sums [splits][M][columns] in ws (no bias, y unused)
 };
 // y = x W^T + bias for few rows (mx4.hip): mx4_few_rows says whether (non-zero) it is the kernel for a product
 int mx4_few_rows(int M, int N, int K);
@@ -412,7 +413,7 @@ struct Mx4Plan {
   int bm, tn, splits;  // rows and 64-column strips of a tile, workgroups that share a tile's reduction
   int dense;
 };
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx);
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits = 32, bool dense = true);
 long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad);
 void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);
 bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx);

@@ -214,6 +214,69 @@ __global__ __launch_bounds__(1024) void ce_pieces_loss_kernel(const float* __res
   }
 }
 
+// ---- few rows on a 4-bit table: fp32 logits of a piece from the 4-bit tiles, these two kernels, the 4-bit gradient tiles.
+// (row, 2,048 columns) per workgroup: maximum and sum of exp(l - maximum)
+constexpr int kChunk = 2048;
+__global__ __launch_bounds__(256) void ce_few_stats_kernel(const float* __restrict__ logits, int W,
+                                                           float2* __restrict__ stats) {
+  __shared__ float red[16];
+  const float* l = logits + (long)blockIdx.y * W;
+  const int c0 = blockIdx.x * kChunk;
+  float v[kChunk / 256], m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kChunk / 256; ++i) {
+    const int c = c0 + i * 256 + threadIdx.x;
+    v[i] = c < W ? l[c] : -INFINITY;
+    m = fmaxf(m, v[i]);
+  }
+  m = block_max(m, red);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kChunk / 256; ++i) s += v[i] == -INFINITY ? 0.f : __expf(v[i] - m);
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) stats[(long)blockIdx.y * gridDim.x + blockIdx.x] = float2{m, s};
+}
+
+// The row's running maximum and sum over the pieces so far (old state -> new state, by the row's first workgroup), the
+// label's logit, and with E: exp(l - maximum), 0 at the label's column and past the piece's end.
+__global__ __launch_bounds__(256) void ce_few_exp_kernel(const float* __restrict__ logits, int W,
+                                                         const float2* __restrict__ stats, const int64_t* __restrict__ labels,
+                                                         int v0, const float* __restrict__ old_m, const float* __restrict__ old_s,
+                                                         float* __restrict__ run_m, float* __restrict__ run_s,
+                                                         float* __restrict__ lbl, float* __restrict__ accscale,
+                                                         bf16_t* __restrict__ E, long lde) {
+  __shared__ float red[16];
+  const int R = blockIdx.y, C = gridDim.x;
+  const float2* st = stats + (long)R * C;
+  const float m0 = old_m[R];
+  float m = m0;
+  for (int i = threadIdx.x; i < C; i += 256) m = fmaxf(m, st[i].x);
+  m = block_max(m, red);
+  const long rel = labels[R] - v0;
+  const float* l = logits + (long)R * W;
+  if (blockIdx.x == 0) {
+    float s = 0.f;
+    for (int i = threadIdx.x; i < C; i += 256) s += st[i].y == 0.f ? 0.f : st[i].y * __expf(st[i].x - m);
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) {
+      const float back = m0 == -INFINITY ? 0.f : __expf(m0 - m);
+      run_m[R] = m;
+      run_s[R] = old_s[R] * back + s;
+      accscale[R] = back;
+      if (rel >= 0 && rel < W) lbl[R] = l[rel];
+    }
+  }
+  if (!E) return;
+  const int c0 = blockIdx.x * kChunk;
+#pragma unroll
+  for (int i = 0; i < kChunk / 512; ++i) {  // pairs of columns
+    const int c = c0 + (i * 256 + threadIdx.x) * 2;
+    if (c >= lde) continue;
+    const float a = c < W && c != rel ? __expf(l[c] - m) : 0.f, b = c + 1 < W && c + 1 != rel ? __expf(l[c + 1] - m) : 0.f;
+    *reinterpret_cast<uint32_t*>(E + R * lde + c) = pack_bf2(a, b);
+  }
+}
+
 // rows of the operand copied with zero padding: out [rows, kpad], in [rows_in >= .., K] (ragged last piece)
 __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict__ in, long ldi, long rows_in, int K,
                                                        bf16_t* __restrict__ out, long rows, int kpad) {
@@ -238,6 +301,7 @@ int num_cus() {
 }
 
 struct Layout {
+  float *logits;
   float *run_m, *run_s, *lbl, *zero, *accscale, *counts, *stats, *ratio, *fin, *slab, *acc;
   int64_t* rel;
   bf16_t *E, *wb;
@@ -250,13 +314,22 @@ struct Plan {
   int n;          // pieces
   int splits;     // of a full piece's dgrad
   bool copy_all, copy_last;  // the table's pieces pass through the bf16 workspace
+  bool few;       // few rows on a 4-bit table: no bf16 workspace, the 4-bit tiles
 };
 
+// Rows up to which a 4-bit table is multiplied as it is, loss and gradient in us there / through the bf16 workspace:
+// 262144 x 640 1 row 115 / 240, 64 rows 167 / 250, 256 rows 469 / 474; 262144 x 1152 256 rows 540 / 710; 50257 x 768 256 rows 138 / 143.
+constexpr int kFewRows = 256;
+
 int up64(int x) { return (x + 63) / 64 * 64; }
+
+// the slabs of a few-rows gradient product over w columns of the vocabulary
+Mx4Plan few_plan(const CePiecesArgs& a, int w) { return mx4_plan(a.M, w, a.K, true, up64(w), 32, false); }
 
 Plan make_plan(const CePiecesArgs& a) {
   Plan p{};
   p.width = std::min(a.piece, (a.V + 255) / 256 * 256);
+  p.few = !a.W && a.M <= kFewRows && a.K >= 128;
   p.n = (a.V + p.width - 1) / p.width;
   p.last = a.V - (p.n - 1) * p.width;
   p.copy_all = !a.W || a.K != a.Kp;
@@ -265,19 +338,46 @@ Plan make_plan(const CePiecesArgs& a) {
   return p;
 }
 
+// bump allocation in the workspace (base null: sizes only), 256-byte aligned
+struct Bump {
+  char* base;
+  long o = 0;
+  char* take(long bytes) {
+    char* q = base ? base + o : nullptr;
+    o += (bytes + 255) / 256 * 256;
+    return q;
+  }
+  float* floats(long n) { return reinterpret_cast<float*>(take(n * 4)); }
+};
+
+Layout few_layout(const CePiecesArgs& a, const Plan& p) {
+  const long M = a.M;
+  Bump b{reinterpret_cast<char*>(a.ws)};
+  Layout L{};
+  L.run_m = b.floats(2 * M), L.run_s = b.floats(2 * M);  // old and new, by turns
+  L.lbl = b.floats(M), L.zero = b.floats(M), L.accscale = b.floats(M), L.counts = b.floats((M + 1023) / 1024);
+  L.rel = reinterpret_cast<int64_t*>(b.take(M * 8));
+  L.stats = b.floats(2 * M * ((p.width + kChunk - 1) / kChunk));
+  L.logits = b.floats(M * (long)p.width);
+  if (a.dh) {
+    const long S = std::max(few_plan(a, p.width).splits, few_plan(a, p.last).splits);
+    L.slab = b.floats(S * M * a.K);
+    L.acc = b.floats(M * a.K);
+    L.E = reinterpret_cast<bf16_t*>(b.take(M * (long)p.width * 2));
+  }
+  L.bytes = b.o;
+  return L;
+}
+
 Layout make_layout(const CePiecesArgs& a, const Plan& p) {
   const long M = a.M, T = p.width / 256, mpad = (M + 255) / 256 * 256;
   // the last piece may split otherwise than the full ones
   const long S = std::max(p.splits, a.dh ? ce_dgrad_splits(a.M, a.K, up64(p.last)) : 1);
   Layout L{};
-  long o = 0;
-  char* base = reinterpret_cast<char*>(a.ws);
-  auto take = [&](long bytes) {
-    char* q = base ? base + o : nullptr;
-    o += (bytes + 255) / 256 * 256;
-    return q;
-  };
-  auto floats = [&](long n) { return reinterpret_cast<float*>(take(n * 4)); };
+  if (p.few) return few_layout(a, p);
+  Bump b{reinterpret_cast<char*>(a.ws)};
+  auto take = [&](long bytes) { return b.take(bytes); };
+  auto floats = [&](long n) { return b.floats(n); };
   L.run_m = floats(M), L.run_s = floats(M), L.lbl = floats(M), L.zero = floats(M), L.accscale = floats(M);
   L.counts = floats((M + 1023) / 1024);
   L.rel = reinterpret_cast<int64_t*>(take(M * 8));
@@ -290,7 +390,7 @@ Layout make_layout(const CePiecesArgs& a, const Plan& p) {
     L.E = reinterpret_cast<bf16_t*>(take(M * (long)p.width * 2));
   }
   if (p.copy_last) L.wb = reinterpret_cast<bf16_t*>(take((long)std::min(p.width, p.copy_all && p.n > 1 ? p.width : up64(p.last)) * a.Kp * 2));
-  L.bytes = o;
+  L.bytes = b.o;
   return L;
 }
 
@@ -320,8 +420,35 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
   // rows per workgroup of the finalize: fewer while the workgroups do not fill the chip twice
   int rb = 64;
   for (; rb > 4 && (a.M + rb - 1) / rb < 2 * num_cus(); rb /= 2) {}
-  int last_slabs = 0;
-  for (int i = 0; i < p.n; ++i) {
+  int last_slabs = 0, state = 0;
+  for (int i = 0; p.few && i < p.n; ++i) {
+    const int v0 = i * p.width, w = i + 1 < p.n ? p.width : p.last, C = (w + kChunk - 1) / kChunk;
+    Mx4LinearArgs f{};
+    f.codes = a.codes + (long)v0 * (a.K / 2); f.scales = a.scales + (long)v0 * (a.K / 32);
+    f.x = a.h; f.ldx = a.ldh;
+    f.M = a.M; f.N = w; f.K = a.K;
+    f.ws = L.logits;
+    f.slabs_only = 1;
+    mx4_tiles(f, mx4_plan(a.M, w, a.K, false, a.ldh, 1, false), false, st);
+    ce_few_stats_kernel<<<dim3(C, a.M), 256, 0, st>>>(L.logits, w, reinterpret_cast<float2*>(L.stats));
+    const long o = (long)state * a.M, n = (long)(state ^ 1) * a.M;
+    state ^= 1;
+    ce_few_exp_kernel<<<dim3(C, a.M), 256, 0, st>>>(L.logits, w, reinterpret_cast<const float2*>(L.stats), a.labels, v0, L.run_m + o,
+                                                    L.run_s + o, L.run_m + n, L.run_s + n, L.lbl, L.accscale,
+                                                    grad ? L.E : nullptr, up64(w));
+    if (!grad) continue;
+    f.x = L.E; f.ldx = up64(w);
+    f.ws = L.slab;
+    const Mx4Plan dp = few_plan(a, w);
+    mx4_tiles(f, dp, true, st);
+    if (i + 1 == p.n) {
+      last_slabs = dp.splits;
+      break;
+    }
+    const long n4 = (long)a.M * a.K / 4;
+    ce_piece_merge_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(L.slab, dp.splits, a.M, a.K, i ? L.accscale : nullptr, L.acc);
+  }
+  for (int i = 0; !p.few && i < p.n; ++i) {
     const int v0 = i * p.width, w = i + 1 < p.n ? p.width : p.last, wp = up64(w), T = (wp + 255) / 256;
     const bf16_t* W = a.W ? a.W + (long)v0 * a.ldw : nullptr;
     long ldw = a.ldw;
@@ -378,7 +505,7 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
   }
   auto rk = last_slabs >= 8 ? ce_pieces_rows_kernel<4> : ce_pieces_rows_kernel<1>;
   rk<<<last_slabs >= 8 ? a.M : (a.M + 3) / 4, 256, 0, st>>>(
-      L.run_m, L.run_s, L.lbl, a.labels, a.M, a.K, a.V, L.counts, last_slabs && p.n == 1 ? nullptr : L.acc,
+      L.run_m + (long)state * a.M, L.run_s + (long)state * a.M, L.lbl, a.labels, a.M, a.K, a.V, L.counts, last_slabs && p.n == 1 ? nullptr : L.acc,
       last_slabs ? L.accscale : nullptr, L.slab, last_slabs, a.W, a.ldw, a.codes, a.scales, a.loss_rows, a.dh);
   ce_pieces_loss_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.M, L.counts, a.loss, a.n_valid);
 }

@@ -373,11 +373,12 @@ void launch_k(const Mx4LinearArgs& a, const Mx4Plan& p, hipStream_t st) {
 
 template <int BM, int TN>
 void launch(const Mx4LinearArgs& a, const Mx4Plan& p, bool dg, hipStream_t st) {
+  const bool part = p.splits > 1 || a.slabs_only;
   if (dg) {
-    if (p.splits > 1) launch_k<BM, TN, true, true>(a, p, st);
+    if (part) launch_k<BM, TN, true, true>(a, p, st);
     else launch_k<BM, TN, true, false>(a, p, st);
   } else {
-    if (p.splits > 1) launch_k<BM, TN, false, true>(a, p, st);
+    if (part) launch_k<BM, TN, false, true>(a, p, st);
     else launch_k<BM, TN, false, false>(a, p, st);
   }
 }
@@ -403,7 +404,7 @@ constexpr TileCost kCostDx[] = {{128, 4, 1.28f, 0.78f, 3.5f}, {128, 2, 0.81f, 0.
 
 }  // namespace
 
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx) {
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits, bool dense) {
   if (K < 128) return Mx4Plan{64, 2, 1, 0};  // the narrow kernel
   const long cols = dgrad ? K : N, red = dgrad ? N : K;
   const long steps = dgrad ? (red + 63) / 64 : (red + 127) / 128;
@@ -412,7 +413,7 @@ Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx) {
   auto consider = [&](const TileCost& c) {
     if (M <= c.bm / 2 && c.bm > 32) return;  // (32 rows: the smallest dx tile)
     const long tiles = (M + c.bm - 1L) / c.bm * ((cols + 64 * c.tn - 1) / (64 * c.tn));
-    for (int s = 1; s <= 32; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : 8) {
+    for (int s = 1; s <= max_splits; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : 8) {
       if (s > 1 && (steps / s < 2 || tiles * s > 2048)) break;
       const double n = (double)((tiles * s + 255) / 256), per = (double)((steps + s - 1) / s);
       double t = (dgrad ? 2.6 : 3.0) + per * std::max((double)c.lat, n * c.thr) + n * c.fix;
@@ -426,7 +427,7 @@ Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx) {
     for (const TileCost& c : kCostY) consider(c);
   // through a bf16 copy: its writing and reading at 4.5 TB/s, then 256 x 256 tiles of gemm4 in K steps of 64 -- 1.15 us alone
   // on a CU, 1.5 us when every CU is busy -- and about 4 us per round of tiles
-  if (mx4_dense_supported(M, N, K, dgrad, ldx)) {
+  if (dense && mx4_dense_supported(M, N, K, dgrad, ldx)) {
     const double tiles = (double)((M + 255L) / 256 * ((cols + 255) / 256)), rounds = std::ceil(tiles / 256), st = red / 64.0;
     const double t = 5 + (double)N * K * 2.53 / 4.5e6 + std::max(rounds * (st * 1.15 + 4), tiles / 256 * (st * 1.5 + 1));
     if (t < best_t) best = Mx4Plan{0, 0, 1, 1};
@@ -472,13 +473,13 @@ void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t
   else if (shape == 641) launch<64, 1>(a, p, dgrad, st);
   else if (shape == 322) launch<32, 2>(a, p, dgrad, st);
   else if (shape == 321) launch<32, 1>(a, p, dgrad, st);
-  else if (shape == 161 && !dgrad && p.splits > 1) launch_k<16, 1, false, true>(a, p, st);
+  else if (shape == 161 && !dgrad && (p.splits > 1 || a.slabs_only)) launch_k<16, 1, false, true>(a, p, st);
   else if (shape == 161 && !dgrad) launch_k<16, 1, false, false>(a, p, st);
   else {
     fprintf(stderr, "mft::mx4_tiles: no kernel for tile %d x %d\n", p.bm, 64 * p.tn);
     abort();
   }
-  if (p.splits > 1) {
+  if (p.splits > 1 && !a.slabs_only) {
     const int cols = dgrad ? a.K : a.N;
     const long n = (long)a.M * cols;
     const bf16_t* bias = dgrad ? nullptr : a.bias;

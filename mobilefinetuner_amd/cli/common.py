@@ -93,6 +93,21 @@ def add_runtime_args(ap):
     g.add_argument("--dist_timeout_s", type=float, default=600.0, help="collective timeout (RCCL watchdog)")
 
 
+def add_base_args(ap):
+    g = ap.add_argument_group("base weights")
+    g.add_argument("--base_mx4", action="store_true",
+                   help="hold the frozen base (projections and vocabulary table) in 4 bits (peft.mx4.quantize_base); "
+                        "adapters are trained and applied on top, never merged")
+
+
+def quantize_base(a, model):
+    """--base_mx4, after the base weights are final."""
+    if not a.base_mx4:
+        return
+    from ..peft.mx4 import quantize_base as q
+    log0(f"  ✓ Base in 4 bits: {q(model) / 1e6:.1f} MB")
+
+
 def runtime_train_kwargs(a) -> dict:
     """TrainConfig fields fed from the runtime flag block."""
     return dict(profile_steps=getattr(a, "profile_steps", ""),

@@ -23,6 +23,7 @@ def build_parser():
     ap.add_argument("--model_type", default="gpt2", choices=["gpt2", "gemma"])
     ap.add_argument("--tokenizer_dir", default="")
     common.add_runtime_args(ap)
+    common.add_base_args(ap)
     return ap
 
 
@@ -48,9 +49,14 @@ def main(argv=None):
     if a.lora_path:
         t, m = load_lora(a.lora_path)
         attach_lora(model, t, m)
-        if a.lora_merge:
+        if a.lora_merge and not a.base_mx4:
             merge_all(model)
             set_lora_enabled(model, False)
+        elif a.base_mx4 and dev.type == "cuda":  # a separate adapter: bf16 compute shadows of its fp32 A / B
+            from ..peft.lora import lora_parameters
+            from ..utils.params import FlatParams
+            model._lora_flat = FlatParams(lora_parameters(model), dev)
+    common.quantize_base(a, model)
     data = read_split(a.mmlu_root, a.split)
     log0(f"[eval_mmlu] {sum(len(v) for v in data.values())} questions in {len(data)} subjects (split={a.split}, "
          f"fewshot={a.fewshot})")

@@ -36,6 +36,7 @@ def build_parser():
     ap.add_argument("--pretokenized_meta", default="")
     ap.add_argument("--max_batches", type=int, default=0)
     common.add_runtime_args(ap)
+    common.add_base_args(ap)
     return ap
 
 
@@ -79,7 +80,7 @@ def main(argv=None):
         tensors, meta = load_lora(a.lora_path)
         spec = attach_lora(model, tensors, meta)
         log0(f"  ✓ LoRA attached: rank={spec.rank} alpha={spec.alpha:g}")
-        if a.lora_merge:
+        if a.lora_merge and not a.base_mx4:
             merge_all(model)
             set_lora_enabled(model, False)
             log0("  ✓ LoRA merged into base weights")
@@ -88,6 +89,7 @@ def main(argv=None):
             from ..peft.lora import lora_parameters
             from ..utils.params import FlatParams
             model._lora_flat = FlatParams(lora_parameters(model), dev)
+    common.quantize_base(a, model)
     if a.model_type == "gemma":
         eos = model.cfg.eos_token_id
     else:

@@ -53,6 +53,7 @@ def build_parser():
     common.add_energy_args(ap)
     common.add_shard_args(ap)
     common.add_runtime_args(ap)
+    common.add_base_args(ap)
     return ap
 
 
@@ -98,6 +99,7 @@ def main(argv=None):
         from ..parallel.sharder import shard_gpt2
         sh = shard_gpt2(model, a.shard_budget_mb << 20, a.shard_dir)
         log0(f"  ✓ Parameter sharding ON: budget={a.shard_budget_mb} MB, host tier {sh.tier.host_bytes >> 20} MB")
+    common.quantize_base(a, model)
     flat = FlatParams(lora_parameters(model), dev)
     log0(f"  trainable params: {flat.numel:,} (padded)  |  total: {model.num_parameters():,}")
 

@@ -72,6 +72,7 @@ def build_parser():
     common.add_energy_args(ap)
     common.add_shard_args(ap)
     common.add_runtime_args(ap)
+    common.add_base_args(ap)
     return ap
 
 
@@ -171,6 +172,7 @@ def main(argv=None):
         budget = max(a.shard_budget_mb << 20, 2 * largest)  # reference raises the budget to the largest param
         sh = shard_gemma(model, budget, a.shard_dir)
         log0(f"  ✓ Parameter sharding ON: budget={budget >> 20} MB")
+    common.quantize_base(a, model)
     flat = FlatParams(lora_parameters(model), dev)
     cfg = model.cfg
     dcfg = WT2Config(data_dir=a.data_dir, seq_len=a.seq_len, eos_id=cfg.eos_token_id, pad_id=cfg.pad_token_id,

@@ -90,7 +90,7 @@ def score_prompts(model, tokenizer, prompts, letter_ids, device, batch_size=16, 
             last.append(r * L + len(enc[i]) - 1)
         h = model.hidden(ids.to(device))
         hl = h[torch.tensor(last, device=device)]
-        logits = hl @ w.t()
+        logits = Fx.mx4_linear(hl, w) if isinstance(w, Fx.MX4Weight) else hl @ w.t()
         if logits.is_cuda and logits.dtype == torch.bfloat16:
             lp = native().logsoftmax_gather(logits.contiguous(), idx, V).float().cpu()
         else:

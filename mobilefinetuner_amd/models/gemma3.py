@@ -25,7 +25,7 @@ import torch.nn as nn
 from ..ops import functional as Fx
 from ..ops.rope_tables import rope_tables
 from ..parallel.sharder import gate
-from .layers import Linear, RMSNorm
+from .layers import Linear, RMSNorm, mx4_weights, refuse_mx4
 
 
 def _pattern_layer_types(n_layers: int, pattern: int = 6):
@@ -262,7 +262,8 @@ class Gemma3Model(nn.Module):
     def logits(self, input_ids, kv_lens=None):
         h = self.hidden(input_ids, kv_lens)
         w = Fx.cw(self.embed)
-        return (h @ w.t())[:, : self.cfg.vocab_size].view(*input_ids.shape, -1)
+        y = Fx.mx4_linear(h, w) if isinstance(w, Fx.MX4Weight) else h @ w.t()
+        return y[:, : self.cfg.vocab_size].view(*input_ids.shape, -1)
 
     def nll(self, input_ids, labels, kv_lens=None):
         h = self.hidden(input_ids, kv_lens)
@@ -272,9 +273,11 @@ class Gemma3Model(nn.Module):
         ps = [p for p in self.parameters() if (p.requires_grad or not trainable_only)]
         n = sum(p.numel() for p in ps)
         if not trainable_only:
+            n += sum(w.numel() for w in mx4_weights(self))
             n -= (self.cfg.vocab_padded - self.cfg.vocab_size) * self.cfg.hidden_size
         return n
 
     def set_full_finetune(self):
+        refuse_mx4(self, "set_full_finetune")
         for p in self.parameters():
             p.requires_grad_(True)

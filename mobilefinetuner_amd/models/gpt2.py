@@ -21,7 +21,7 @@ import torch.nn as nn
 
 from ..ops import functional as Fx
 from ..parallel.sharder import gate
-from .layers import LayerNorm, Linear
+from .layers import LayerNorm, Linear, mx4_weights, refuse_mx4
 
 
 @dataclass
@@ -198,7 +198,8 @@ class GPT2Model(nn.Module):
     def logits(self, input_ids, kv_lens=None):
         h = self.hidden(input_ids, kv_lens)
         w = Fx.cw(self.wte)
-        return (h @ w.t())[:, : self.cfg.vocab_size].view(*input_ids.shape, -1)
+        y = Fx.mx4_linear(h, w) if isinstance(w, Fx.MX4Weight) else h @ w.t()
+        return y[:, : self.cfg.vocab_size].view(*input_ids.shape, -1)
 
     def nll(self, input_ids, labels, kv_lens=None):
         """(sum NLL, #tokens) over shifted labels — token-weighted eval."""
@@ -209,9 +210,11 @@ class GPT2Model(nn.Module):
         ps = [p for p in self.parameters() if (p.requires_grad or not trainable_only)]
         n = sum(p.numel() for p in ps)
         if not trainable_only:
+            n += sum(w.numel() for w in mx4_weights(self))
             n -= (self.cfg.vocab_padded - self.cfg.vocab_size) * self.cfg.n_embd
         return n
 
     def set_full_finetune(self):
+        refuse_mx4(self, "set_full_finetune")
         for p in self.parameters():
             p.requires_grad_(True)

@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import torch
 
+from .layers import refuse_mx4
+
 
 def _strip(sd):
     out = {}
@@ -29,6 +31,7 @@ def _put(param, value):
 @torch.no_grad()
 def load_gpt2_state(model, sd: dict):
     """sd: HF GPT2 state dict (torch tensors); missing keys raise."""
+    refuse_mx4(model, "load_gpt2_state")
     sd = _strip(sd)
     V, C = model.cfg.vocab_size, model.cfg.n_embd
     wte = sd["wte.weight"]
@@ -56,6 +59,7 @@ def load_gpt2_state(model, sd: dict):
 @torch.no_grad()
 def export_gpt2_state(model, prefix: str = "") -> dict:
     """HF-keyed fp32 state dict (Conv1D [in,out] layout) — the full-FT checkpoint format."""
+    refuse_mx4(model, "export_gpt2_state")
     V = model.cfg.vocab_size
     f = lambda t: t.detach().float().cpu().contiguous()  # noqa: E731
     sd = {prefix + "wte.weight": f(model.wte[:V]), prefix + "wpe.weight": f(model.wpe)}
@@ -81,6 +85,7 @@ def export_gpt2_state(model, prefix: str = "") -> dict:
 @torch.no_grad()
 def load_gemma_state(model, sd: dict):
     """sd: HF Gemma3ForCausalLM / Gemma3TextModel state dict."""
+    refuse_mx4(model, "load_gemma_state")
     def g(k):
         for cand in (k, "model." + k, "model.language_model." + k, "language_model.model." + k):
             if cand in sd:
@@ -111,6 +116,7 @@ def load_gemma_state(model, sd: dict):
 
 @torch.no_grad()
 def export_gemma_state(model, prefix: str = "model.") -> dict:
+    refuse_mx4(model, "export_gemma_state")
     cfg = model.cfg
     f = lambda t: t.detach().float().cpu().contiguous()  # noqa: E731
     qd, kd = cfg.num_attention_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim

@@ -13,12 +13,23 @@ import torch
 import torch.nn as nn
 
 from ..ops import functional as Fx
+from ..ops.mx4 import MX4Weight
 
 
 def _salt(name: str) -> int:
     """Stable per-adapter salt for the dropout hash (zlib.crc32: not randomised per process)."""
     import zlib
     return zlib.crc32(name.encode())
+
+
+def mx4_weights(model):
+    """The MX4Weights of a model whose base was quantised (peft.mx4.quantize_base)."""
+    return [w for m in model.modules() for w in m.__dict__.values() if isinstance(w, MX4Weight)]
+
+
+def refuse_mx4(model, what: str):
+    if mx4_weights(model):
+        raise RuntimeError(f"{what}: not on a 4-bit base (peft.mx4.quantize_base)")
 
 
 @dataclass
@@ -65,10 +76,12 @@ class Linear(nn.Module):
     def aug_cols(self) -> int:
         """Input width the producer should allocate for the augmented-K LoRA forward
         (ops.functional._LoRALinearAug), or 0 when this Linear takes a plain input: no active
-        adapter, a trainable base weight, CPU tensors, in_features not a multiple of 32, or
+        adapter, a trainable or 4-bit base weight, CPU tensors, in_features not a multiple of 32, or
         MFT_LORA_AUG=0."""
         import os
         if not (self.lora_slices and self.lora_enabled) or self.weight.requires_grad or not self.weight.is_cuda:
+            return 0
+        if isinstance(self.weight, MX4Weight):  # no bf16 copy of a 4-bit weight
             return 0
         if getattr(self.weight, "_mft_sharded", False):  # no resident W copy for offloaded weights
             return 0
@@ -101,6 +114,8 @@ class Linear(nn.Module):
     @torch.no_grad()
     def merge_lora(self, sign: float = 1.0):
         """W[col0:col0+n, :] += sign * s * B^T A  (merge; sign=-1 unmerges) — K10."""
+        if isinstance(self.weight, MX4Weight):
+            raise RuntimeError("merge_lora: a 4-bit base takes no adapter in; keep it separate, or merge before quantising")
         for sl in self.lora_slices:
             A, B = sl.A.detach().float().contiguous(), sl.B.detach().float().contiguous()   # [r, in], [r, n]
             w = self.weight.data

@@ -755,7 +755,8 @@ def fused_mlp_available() -> bool:
 def mlp_gelu(x, fc, proj):
     """GPT-2 MLP: proj(GELU(fc(x))).  Fused-epilogue path when neither Linear carries an active
     LoRA adapter (the adapter's rank-r update lands between the GEMM and the GELU)."""
-    plain = not ((fc.lora_slices and fc.lora_enabled) or (proj.lora_slices and proj.lora_enabled))
+    plain = not (isinstance(fc.weight, MX4Weight) or isinstance(proj.weight, MX4Weight)
+                 or (fc.lora_slices and fc.lora_enabled) or (proj.lora_slices and proj.lora_enabled))
     K = x.shape[-1]
     if (x.is_cuda and plain and fc.bias is not None and proj.bias is not None and fused_mlp_available()
             and K % 64 == 0 and fc.out_features % 64 == 0):

@@ -149,8 +149,14 @@ def gate(x, sharder, name):
     return _Gate.apply(x, sharder, name)
 
 
+def _refuse_mx4(model):
+    from ..models.layers import refuse_mx4
+    refuse_mx4(model, "parameter sharding")
+
+
 def shard_gpt2(model, budget_bytes: int, disk_dir: str = "") -> ParameterSharder:
     """Register GPT-2's frozen weights per block (plus embeddings) and attach to the model."""
+    _refuse_mx4(model)
     sh = ParameterSharder(budget_bytes, disk_dir)
     sh.register_group("embed", [model.wte.data, model.wpe.data])
     for i, b in enumerate(model.blocks):
@@ -164,6 +170,7 @@ def shard_gpt2(model, budget_bytes: int, disk_dir: str = "") -> ParameterSharder
 
 
 def shard_gemma(model, budget_bytes: int, disk_dir: str = "") -> ParameterSharder:
+    _refuse_mx4(model)
     sh = ParameterSharder(budget_bytes, disk_dir)
     sh.register_group("embed", [model.embed.data])
     for i, L in enumerate(model.layers):

@@ -1,0 +1,89 @@
+"""LoRA models on a 4-bit base (peft.mx4.quantize_base): wiring, refusals and CLIs on host tensors (oracle ops)."""
+import os
+
+import pytest
+import torch
+
+CPU = ["--device", "cpu", "--dtype", "fp32", "--random_init", "--synthetic_data", "--synthetic_tokens", "20000"]
+
+
+def _model(kind, quantize=True, lora=True):
+    from mobilefinetuner_amd.peft.lora import LoraSpec, inject_gemma, inject_gpt2
+    from mobilefinetuner_amd.peft.mx4 import quantize_base
+    if kind == "gpt2":
+        from mobilefinetuner_amd.models.gpt2 import GPT2Config, GPT2Model
+        m = GPT2Model(GPT2Config.preset("gpt2-tiny"), dtype=torch.float32, device="cpu", seed=1)
+        if lora:
+            inject_gpt2(m, LoraSpec(rank=8, alpha=16))
+    else:
+        from mobilefinetuner_amd.models.gemma3 import Gemma3Config, Gemma3Model
+        m = Gemma3Model(Gemma3Config.preset("gemma3-tiny"), dtype=torch.float32, device="cpu", seed=1)
+        if lora:
+            inject_gemma(m, LoraSpec(rank=8, alpha=16, targets=["q_proj", "down_proj"], init="peft"))
+    if quantize:
+        quantize_base(m)
+    return m
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "gemma"])
+def test_quantized_model_equals_its_values(kind):
+    """Every base weight is the MX4Weight of the original one, and the model computes with its values: close to the fp32
+    model that holds them (the lookup's bf16 rounding and the bf16 that follows it on the host, 2^-8 a rounding)."""
+    from mobilefinetuner_amd.models.layers import mx4_weights
+    from mobilefinetuner_amd.ops import functional as Fx
+    a, b = _model(kind), _model(kind, quantize=False)
+    assert len(mx4_weights(a)) == len(a.linear_modules()) + 1
+    assert a.num_parameters() == b.num_parameters()
+    name = "wte" if kind == "gpt2" else "embed"
+    with torch.no_grad():
+        for (n, la), (_, lb) in zip(a.linear_modules().items(), b.linear_modules().items()):
+            want = Fx.mx4_quantize(lb.weight.data)
+            assert torch.equal(la.weight.codes, want.codes) and torch.equal(la.weight.scales, want.scales), n
+            lb.weight.copy_(want.dequantize())
+        getattr(b, name).copy_(Fx.mx4_quantize(getattr(b, name).data).dequantize())
+    ids = torch.randint(0, 500, (2, 33), generator=torch.Generator().manual_seed(0))
+    la, lb = a(ids[:, :-1], ids[:, 1:]), b(ids[:, :-1], ids[:, 1:])
+    assert abs(la.item() - lb.item()) < 2.0 ** -7 * lb.item()
+    la.backward()
+    assert all(p.grad is not None for p in a.parameters() if p.requires_grad)
+    with torch.no_grad():
+        assert a.logits(ids[:, :4]).shape == b.logits(ids[:, :4]).shape
+        s, n = a.nll(ids[:, :-1], ids[:, 1:])
+        assert n.item() == 64 and abs(s.item() / 64 - la.item()) < 1e-4
+
+
+def test_refusals():
+    from mobilefinetuner_amd.models import hf_io
+    from mobilefinetuner_amd.parallel.sharder import shard_gpt2
+    from mobilefinetuner_amd.peft.lora import merge_all
+    from mobilefinetuner_amd.peft.mx4 import is_quantized, quantize_base
+    m = _model("gpt2")
+    assert is_quantized(m)
+    with pytest.raises(RuntimeError, match="already"):
+        quantize_base(m)
+    with pytest.raises(RuntimeError, match="4-bit base"):
+        merge_all(m)
+    with pytest.raises(RuntimeError, match="4-bit base"):
+        m.set_full_finetune()
+    with pytest.raises(RuntimeError, match="4-bit base"):
+        hf_io.export_gpt2_state(m)
+    with pytest.raises(RuntimeError, match="4-bit base"):
+        hf_io.load_gpt2_state(m, {})
+    with pytest.raises(RuntimeError, match="4-bit base"):
+        shard_gpt2(m, 1 << 20)
+    full = _model("gpt2", quantize=False, lora=False)
+    full.set_full_finetune()
+    with pytest.raises(RuntimeError, match="trainable"):
+        quantize_base(full)
+
+
+def test_clis(tmp_path):
+    from mobilefinetuner_amd.cli import eval_ppl, gpt2_lora_finetune, train_lora_gemma
+    out = str(tmp_path / "lora.safetensors")
+    tr = gpt2_lora_finetune.main(["--model", "gpt2-tiny", *CPU, "--base_mx4", "--steps", "3", "--batch_size", "2",
+                                  "--seq_len", "32", "--lora_out", out, "--eval_interval", "3", "--eval_batches", "1"])
+    assert len(tr.history) == 3 and os.path.exists(out)
+    tr = train_lora_gemma.main(["--model", "gemma3-tiny", *CPU, "--base_mx4", "--max_steps", "2", "--batch", "2",
+                                "--seq_len", "32", "--output_dir", str(tmp_path), "--targets", "full"])
+    assert len(tr.history) == 2
+    eval_ppl.main(["--model", "gpt2-tiny", *CPU, "--base_mx4", "--seq_len", "32", "--max_batches", "2", "--lora_path", out])

@@ -87,7 +87,8 @@ def _flags(kind: str, incs, abi):
     if kind == "hip":
         # Device code: gfx950 only. -ffp-contract=fast lets hipcc fuse mul+add into v_fma.  Packed fp32
         # (v_pk_add / mul / fma_f32) is off: some of its forms have given wrong results now and then,
-        # without an error; the scalar forms round the same.
+        # without an error.  The scalar forms round alike, but more of the products then fuse into an fma
+        # (the norms' sums, attention's delta, the LoRA updates), so those differ in the last fp32 bits.
         return common + [f"--offload-arch={ARCH}", "-ffp-contract=fast", "-munsafe-fp-atomics", "-fno-gpu-rdc",
                          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     py_inc = sysconfig.get_paths()["include"]

@@ -125,7 +125,7 @@ __device__ __forceinline__ void gelu_tanh_and_grad(float x, float& y, float& dy)
 
 // Two elements at once as float2 arithmetic with the constants folded: ~10 mul / fma per element and 2
 // v_exp_f32 + 2 v_rcp_f32 per pair.  (Compiled to scalar fp32 instructions: the build turns packed fp32
-// off, which costs the headline step 0.6 % and is bit-identical.)
+// off, which costs the headline step 0.6 %.)
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void gelu_tanh_and_grad2(f32x2_t x, f32x2_t& y, f32x2_t& dy) {
   const float k0 = 0.7978845608028654f, k1 = 0.044715f, l2e = 1.4426950408889634f;

@@ -20,6 +20,17 @@ int sumsq_blocks(long n) {
   return (int)(b < 1024 ? b : 1024);
 }
 
+// a * b for a sum.  R: rounded to fp32 by itself (the empty asm hides where it comes from, so the sum cannot
+// take it into an fma); else the compiler may fuse.  Which products are rounded decides the last bit of the
+// moments and the weights: they are fixed here, so that a run repeats bit for bit under another compiler
+// setting, such as packed fp32 on or off.
+template <bool R>
+__device__ __forceinline__ float prod(float a, float b) {
+  float p = a * b;
+  if constexpr (R) asm("" : "+v"(p));
+  return p;
+}
+
 __global__ __launch_bounds__(256) void sumsq_partial_kernel(const float* __restrict__ x, long n, float* __restrict__ part) {
   __shared__ float red[16];
   float s = 0.f;
@@ -27,7 +38,7 @@ __global__ __launch_bounds__(256) void sumsq_partial_kernel(const float* __restr
   const float4* x4 = reinterpret_cast<const float4*>(x);
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {
     const float4 v = x4[i];
-    s += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+    s += prod<true>(v.x, v.x) + prod<true>(v.y, v.y) + prod<true>(v.z, v.z) + prod<true>(v.w, v.w);
   }
   if (blockIdx.x == 0)
     for (long i = n4 * 4 + threadIdx.x; i < n; i += blockDim.x) s += x[i] * x[i];
@@ -152,10 +163,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamWArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float gj = gg[j] * clip;
-        if (a.l2_coupled) gj += a.weight_decay * pp[j];
+        float gj = prod<!MB>(gg[j], clip);
+        if (a.l2_coupled) gj += prod<!MB>(a.weight_decay, pp[j]);
         mm[j] = a.beta1 * mm[j] + (1.f - a.beta1) * gj;
-        vv[j] = a.beta2 * vv[j] + (1.f - a.beta2) * gj * gj;
+        vv[j] = prod<!MB>(a.beta2, vv[j]) + prod<!MB>((1.f - a.beta2) * gj, gj);
         float denom = sqrtf(vv[j]) * rbc2 + a.eps;
         if (!MB && a.vmax) {  // AMSGrad, the reference's rule (optim/adam.cpp:75-80): the running max of
           // the BIAS-CORRECTED second moment, v_hat = max(v_hat, v / bc2), used as is in the denominator
@@ -190,11 +201,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamWArgs a) {
   }
   if (blockIdx.x == 0) {
     for (long i = n4 * 4 + threadIdx.x; i < a.n; i += blockDim.x) {
-      float gj = a.g[i] * clip;
+      float gj = prod<true>(a.g[i], clip);
       float pj = a.p[i];
-      if (a.l2_coupled) gj += a.weight_decay * pj;
-      const float mj = a.beta1 * ld_mom<MB>(a.m, i) + (1.f - a.beta1) * gj;
-      const float vj = a.beta2 * ld_mom<MB>(a.v, i) + (1.f - a.beta2) * gj * gj;
+      if (a.l2_coupled) gj += prod<true>(a.weight_decay, pj);
+      const float m0 = ld_mom<MB>(a.m, i), mg = prod<true>(1.f - a.beta1, gj);
+      const float mj = MB ? prod<true>(a.beta1, m0) + mg : fmaf(a.beta1, m0, mg);
+      const float vj = prod<true>(a.beta2, ld_mom<MB>(a.v, i)) + prod<true>((1.f - a.beta2) * gj, gj);
       float denom = sqrtf(vj) * rbc2 + a.eps;
       if (!MB && a.vmax) {  // AMSGrad (reference rule, as above)
         const float vd = fmaxf(a.vmax[i], vj * (rbc2 * rbc2));

@@ -460,7 +460,7 @@ std::vector<Tensor> lm_head_ce_pieces(Tensor h, c10::optional<Tensor> W, c10::op
                     W->size(1) == K && W->size(0) >= V, what, ": the table must be bf16 [>= vocab_size, C] on h's GPU");
     TORCH_CHECK(K > 0 && K % 8 == 0, what, ": C must be a multiple of 8");
     if (!rows16(*W)) W = W->clone(at::MemoryFormat::Contiguous);
-    a.W = bp(*W); a.ldw = W->stride(0); a.w_rows = W->size(0);
+    a.W = bp(*W); a.ldw = W->stride(0);
   } else {
     TORCH_CHECK(codes.has_value() && scales.has_value(), what, ": a table is needed");
     const auto [N, Kw] = mx4_shape(*codes, *scales, what);

@@ -142,6 +142,9 @@ struct GemmArgs {
   // CE_DGRAD_ACC: ce_acc [M, N] fp32 = ce_acc * ce_accscale[row] + the piece's sum (null scale: = the sum)
   float* ce_acc;
   const float* ce_accscale;
+  // CE_FWD (gemm4) and the CE dgrads: vocabulary rows of B that may be read, where N (K in the dgrad) is padded
+  // past the table's end; 0 = all.  The forward reads zeros there, the dgrad its last row, times E = 0.
+  int b_rows;
 };
 // 256x256 8-phase pipelined GEMM (gemm8.hip); same epilogues.  a_t: A stored [K, M]; b_t: B stored
 // [K, N] (NN data-grad); both: TN weight-grad (use GEMM_EPI_F32ACC with gemm8_pick_ksplit / ws)
@@ -245,8 +248,7 @@ void lm_head_ce(const CeArgs& a, hipStream_t st);
 // The same loss swept in pieces of the vocabulary (ce_pieces.hip): no buffer grows with the vocabulary.
 struct CePiecesArgs {
   const bf16_t* h; long ldh;   // [M, Kp] (Kp = K rounded up to 64, columns K .. Kp - 1 zeros)
-  const bf16_t* W; long ldw;   // [rows, Kp]-readable bf16 table, or null: the 4-bit one
-  long w_rows;                 // rows of W that may be read
+  const bf16_t* W; long ldw;   // [V, K] bf16 table, or null: the 4-bit one
   const uint8_t *codes, *scales;  // the 4-bit table [V, K]
   const int64_t* labels;       // [M]; outside [0, V): an ignored row
   int M, K, Kp, V;

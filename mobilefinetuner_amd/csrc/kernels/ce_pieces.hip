@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void ce_piece_merge_kernel(const float* __rest
 
 // WPR waves per row: its loss and, with dh, its gradient.  The last piece's sum comes in here: S > 0 slabs of a split
 // product (on top of acc * accscale when there were pieces before it), or acc alone.  WPR = 4 (few rows): the waves share
-// the slabs out and wave 0 adds their four sums in order (512 rows, 40 slabs: 29 us by one wave per row).
+// the slabs out and wave 0 adds their four sums in order.
 template <int WPR>
 __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __restrict__ run_m, const float* __restrict__ run_s,
                                                              const float* __restrict__ lbl, const int64_t* __restrict__ labels,
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void ce_few_exp_kernel(const float* __restrict
   }
 }
 
-// rows of the operand copied with zero padding: out [rows, kpad], in [rows_in >= .., K] (ragged last piece)
+// rows of the operand copied with zero padding: in [rows_in, K] -> out [rows, kpad]
 __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict__ in, long ldi, long rows_in, int K,
                                                        bf16_t* __restrict__ out, long rows, int kpad) {
   const int k8 = kpad / 8;
@@ -313,7 +313,7 @@ struct Plan {
   int last;       // columns of the last piece
   int n;          // pieces
   int splits;     // of a full piece's dgrad
-  bool copy_all, copy_last;  // the table's pieces pass through the bf16 workspace
+  bool copy;      // the table's pieces pass through the bf16 workspace: a 4-bit table, C not a multiple of 64 or below 128
   bool few;       // few rows on a 4-bit table: no bf16 workspace, the 4-bit tiles
 };
 
@@ -322,6 +322,22 @@ struct Plan {
 constexpr int kFewRows = 256;
 
 int up64(int x) { return (x + 63) / 64 * 64; }
+
+// Slabs of the gradient product over w columns: K splits that hold whole 256-column tiles.  us = rounds of the 256 CUs x
+// (5 + 2.1 per 64 columns) + the slabs written and read back at 4.5 TB/s, the least of it.  Product and sum at 768 channels,
+// w = 50257: 512 rows 40 splits 66 (18: 91, 9: 147); 4096 rows 9 splits 405 (20: 432); 8192 rows 9 splits 815 (18: 860).
+int dgrad_splits(int M, int K, int w) {
+  const int nk = (w + 63) / 64, tiles = ((M + 255) / 256) * ((K + 255) / 256), cus = num_cus();
+  int best = 1;
+  double best_t = 1e30;
+  for (int sp = 1; sp <= 64 && (sp == 1 || nk / sp >= 16); ++sp) {
+    const int kps = (nk + sp - 1) / sp;
+    if (sp > 1 && (kps % 4 || (long)(sp - 1) * kps >= nk)) continue;
+    const double t = (tiles * sp + cus - 1) / cus * (5 + 2.1 * kps) + (sp > 1 ? (double)sp * M * K * 8 / 4.5e6 : 0);
+    if (t < best_t) best_t = t, best = sp;
+  }
+  return best;
+}
 
 // the slabs of a few-rows gradient product over w columns of the vocabulary
 Mx4Plan few_plan(const CePiecesArgs& a, int w) { return mx4_plan(a.M, w, a.K, true, up64(w), 32, false); }
@@ -332,9 +348,8 @@ Plan make_plan(const CePiecesArgs& a) {
   p.few = !a.W && a.M <= kFewRows && a.K >= 128;
   p.n = (a.V + p.width - 1) / p.width;
   p.last = a.V - (p.n - 1) * p.width;
-  p.copy_all = !a.W || a.K != a.Kp;
-  p.copy_last = p.copy_all || (long)(p.n - 1) * p.width + up64(p.last) > a.w_rows;
-  p.splits = a.dh ? ce_dgrad_splits(a.M, a.K, p.n > 1 ? p.width : up64(p.last)) : 1;
+  p.copy = !a.W || a.K != a.Kp || !gemm4_supported(a.M, p.width, a.Kp, false, false);
+  p.splits = a.dh ? dgrad_splits(a.M, a.K, p.n > 1 ? p.width : up64(p.last)) : 1;
   return p;
 }
 
@@ -372,7 +387,7 @@ Layout few_layout(const CePiecesArgs& a, const Plan& p) {
 Layout make_layout(const CePiecesArgs& a, const Plan& p) {
   const long M = a.M, T = p.width / 256, mpad = (M + 255) / 256 * 256;
   // the last piece may split otherwise than the full ones
-  const long S = std::max(p.splits, a.dh ? ce_dgrad_splits(a.M, a.K, up64(p.last)) : 1);
+  const long S = std::max(p.splits, a.dh ? dgrad_splits(a.M, a.K, up64(p.last)) : 1);
   Layout L{};
   if (p.few) return few_layout(a, p);
   Bump b{reinterpret_cast<char*>(a.ws)};
@@ -389,7 +404,7 @@ Layout make_layout(const CePiecesArgs& a, const Plan& p) {
     L.acc = floats(M * a.K);
     L.E = reinterpret_cast<bf16_t*>(take(M * (long)p.width * 2));
   }
-  if (p.copy_last) L.wb = reinterpret_cast<bf16_t*>(take((long)std::min(p.width, p.copy_all && p.n > 1 ? p.width : up64(p.last)) * a.Kp * 2));
+  if (p.copy) L.wb = reinterpret_cast<bf16_t*>(take((long)(p.n > 1 ? p.width : up64(p.last)) * a.Kp * 2));
   L.bytes = b.o;
   return L;
 }
@@ -452,7 +467,7 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
     const int v0 = i * p.width, w = i + 1 < p.n ? p.width : p.last, wp = up64(w), T = (wp + 255) / 256;
     const bf16_t* W = a.W ? a.W + (long)v0 * a.ldw : nullptr;
     long ldw = a.ldw;
-    if (p.copy_all || (p.copy_last && i + 1 == p.n)) {
+    if (p.copy) {
       if (a.W) {
         const long n8 = (long)wp * (a.Kp / 8);
         pad_rows_kernel<<<(unsigned)((n8 + 255) / 256), 256, 0, st>>>(W, a.ldw, w, a.K, L.wb, wp, a.Kp);
@@ -468,9 +483,10 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
     f.C = grad ? L.E : nullptr; f.ldc = wp;
     f.M = a.M; f.N = wp; f.K = a.Kp; f.alpha = 1.f;
     f.ce_labels = L.rel; f.ce_stats = L.stats; f.ce_lbl = L.lbl; f.ce_V = w;
+    f.b_rows = w;  // the table ends anywhere
     if (gemm4_supported(a.M, wp, a.Kp, false, false)) gemm4x(f, GEMM_EPI_CE_FWD, false, false, st);
     else gemm8x(f, GEMM_EPI_CE_FWD, false, false, st);
-    const int S = grad ? ce_dgrad_splits(a.M, a.K, wp) : 1;
+    const int S = grad ? dgrad_splits(a.M, a.K, wp) : 1;
     const int tps = S > 1 ? ((wp / 64 + S - 1) / S) / 4 : T;
     auto fk = rb == 64   ? ce_piece_finalize_kernel<64>
               : rb == 32 ? ce_piece_finalize_kernel<32>
@@ -487,6 +503,7 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
     d.B = W; d.ldb = ldw;
     d.M = a.M; d.N = a.K; d.K = wp; d.alpha = 1.f;
     d.ce_labels = L.rel; d.ce_ratio = L.ratio; d.ce_fin = L.fin; d.ce_wlab = L.zero;
+    d.b_rows = w;
     if (S > 1) {
       d.ksplit = S;
       d.ws = L.slab;
@@ -503,8 +520,9 @@ void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st) {
       gemm8x(d, GEMM_EPI_CE_DGRAD_ACC, false, true, st);
     }
   }
-  auto rk = last_slabs >= 8 ? ce_pieces_rows_kernel<4> : ce_pieces_rows_kernel<1>;
-  rk<<<last_slabs >= 8 ? a.M : (a.M + 3) / 4, 256, 0, st>>>(
+  const bool w4 = last_slabs >= 8 && a.M < 2048;
+  auto rk = w4 ? ce_pieces_rows_kernel<4> : ce_pieces_rows_kernel<1>;
+  rk<<<w4 ? a.M : (a.M + 3) / 4, 256, 0, st>>>(
       L.run_m + (long)state * a.M, L.run_s + (long)state * a.M, L.lbl, a.labels, a.M, a.K, a.V, L.counts, last_slabs && p.n == 1 ? nullptr : L.acc,
       last_slabs ? L.accscale : nullptr, L.slab, last_slabs, a.W, a.ldw, a.codes, a.scales, a.loss_rows, a.dh);
   ce_pieces_loss_kernel<<<1, 1024, 0, st>>>(a.loss_rows, a.M, L.counts, a.loss, a.n_valid);

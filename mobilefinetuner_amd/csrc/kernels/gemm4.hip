@@ -646,7 +646,8 @@ __global__ __launch_bounds__(256, 1) void gemm4p_nt_kernel(GemmArgs g) {
   auto srd_b = [&](int n0) {
     if constexpr (EPI == GEMM_EPI_GEGLU_FWD)  // rows n0 / 2 .. of the gate half, the up half I rows further
       return make_srd(g.B + (long)(n0 >> 1) * g.ldb, (uint32_t)min((long)(2 * g.geglu_I - (n0 >> 1)) * g.ldb * 2, 0xffffffffL));
-    return make_srd(g.B + (long)n0 * g.ldb, PDIAG == 2 ? 0u : (uint32_t)min((long)(g.N - n0) * g.ldb * 2, 0xffffffffL));
+    const int nr = EPI == GEMM_EPI_CE_FWD && g.b_rows ? g.b_rows : g.N;
+    return make_srd(g.B + (long)n0 * g.ldb, PDIAG == 2 ? 0u : (uint32_t)min((long)(nr - n0) * g.ldb * 2, 0xffffffffL));
   };
   auto srd_a2 = [&](int m0) {
     return make_srd(g.A2 + (long)m0 * g.lda2, (uint32_t)min((long)(g.M - m0) * g.lda2 * 2, 0xffffffffL));

@@ -127,7 +127,10 @@ __device__ __forceinline__ void stage_half_fast(bf16_t* lds, const bf16_t* src, 
 // bank slots -> conflict-free transposed reads.
 __device__ __forceinline__ int tsw(int k) { return ((k & 3) | (((k >> 3) & 1) << 2)) << 1; }
 
-__device__ __forceinline__ void stage_half_t(bf16_t* lds, const bf16_t* src, long ld, int c0, int cmax, int k0) {
+// KC: rows past kmax - 1 read row kmax - 1
+template <bool KC = false>
+__device__ __forceinline__ void stage_half_t(bf16_t* lds, const bf16_t* src, long ld, int c0, int cmax, int k0,
+                                             int kmax = 0) {
   const int tid = threadIdx.x, w = tid >> 6;
   const int cb = min(c0, cmax - 8);
   const bf16_t* base = src + (long)k0 * ld + cb;
@@ -136,7 +139,8 @@ __device__ __forceinline__ void stage_half_t(bf16_t* lds, const bf16_t* src, lon
     const int c = t * 512 + tid;
     const int r = c >> 4, s = c & 15;
     const int gc = min(c0 + ((s ^ tsw(r)) << 3), cmax - 8) - cb;
-    glds16_off(base, (uint32_t)((r * (int)ld + gc) * 2), lds + (t * 512 + w * 64) * 8);
+    const int gr = KC ? min(r, kmax - 1 - k0) : r;
+    glds16_off(base, (uint32_t)((gr * (int)ld + gc) * 2), lds + (t * 512 + w * 64) * 8);
   }
 }
 
@@ -750,7 +754,8 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
       if constexpr (AT) stage_half_t(half_ptr(buf, h), g.A, g.lda, m0 + h * 128, g.M, k0);
       else stage_half(half_ptr(buf, h), g.A, g.lda, m0 + h * 128, g.M, k0);
     } else {
-      if constexpr (BT) stage_half_t(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0);
+      if constexpr (kCeDgrad<EPI>) stage_half_t<true>(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0, g.b_rows ? g.b_rows : g.K);
+      else if constexpr (BT) stage_half_t(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0);
       else stage_half(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0);
     }
   };

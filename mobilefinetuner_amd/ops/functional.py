@@ -1180,8 +1180,8 @@ def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
     them, are ignored; none at all gives 0), swept in pieces of ``piece`` vocabulary columns (a multiple of
     256; None: a size from the row count): beside h, dh and an fp32 dh the memory is one [rows, piece] bf16
     buffer, whatever the vocabulary -- lm_head_cross_entropy keeps one of the whole vocabulary's width.  W is
-    frozen: bf16 [>= vocab_size, C] (C a multiple of 8; padding rows, read up to the next multiple of 64, must be
-    finite) or an MX4Weight; the gradient goes to h.  A trainable W is lm_head_cross_entropy's."""
+    frozen: bf16 [>= vocab_size, C] (C a multiple of 8; rows past the vocabulary are not used) or
+    an MX4Weight; the gradient goes to h.  A trainable W is lm_head_cross_entropy's."""
     if _needs(w):
         raise RuntimeError("lm_head_cross_entropy_pieces: W is frozen here; lm_head_cross_entropy trains it")
     piece = int(piece or 0)

@@ -275,3 +275,15 @@ def test_refusals():
         Fx.lm_head_cross_entropy_pieces(h[:, :20], w[:, :20], labels, 300)
     with pytest.raises(RuntimeError, match="frozen"):
         Fx.lm_head_cross_entropy_pieces(h, w.clone().requires_grad_(True), labels, 300)
+
+
+@pytest.mark.parametrize("m,k,v,piece", [(200, 128, 1000, None), (40, 64, 1000, None), (40, 96, 1001, 512), (300, 768, 50257, 8192),
+                                         (2100, 256, 9999, None)])
+def test_memory_after_the_vocabulary_is_not_used(m, k, v, piece):
+    """The table ends inside a 64-row block: what lies after its rows, NaN here, reaches neither loss nor gradient."""
+    h, w, wd, labels = _case(m, k, v, "bf16", seed=9)
+    buf = torch.full((v + 300, k), float("nan"), device="cuda", dtype=torch.bfloat16)
+    buf[:v] = w
+    loss, dh = _check(h, buf[:v], wd, labels, v, piece)
+    again, dh2 = _run(h, buf, labels, v, piece)
+    assert torch.equal(loss, again) and torch.equal(dh, dh2)

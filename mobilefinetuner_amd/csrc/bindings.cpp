@@ -439,6 +439,22 @@ Tensor mx4_linear(Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> b
 }
 Tensor mx4_dgrad(Tensor dy, Tensor codes, Tensor scales) { return mx4_product(dy, codes, scales, c10::nullopt, true); }
 
+// mx4_linear with its gradient to x as a node of the autograd graph in C++: forward and backward take 29 us of the host,
+// 58 us through a python Function, while the products of a 512 x 2304 x 768 step take 23 us.
+struct MX4LinearNode : public torch::autograd::Function<MX4LinearNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> bias) {
+    ctx->save_for_backward({codes, scales});
+    return mx4_product(x, codes, scales, bias, false);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dy) {
+    const auto w = ctx->get_saved_variables();
+    return {mx4_product(dy[0], w[0], w[1], c10::nullopt, true), Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor mx4_linear_grad(Tensor x, Tensor codes, Tensor scales, c10::optional<Tensor> bias) {
+  return MX4LinearNode::apply(x, codes, scales, bias);
+}
+
 // LM-head cross entropy in pieces of the vocabulary (ce_pieces.hip): h [M, K], the table bf16 [>= V, K] or 4-bit
 // [V, K].  Returns {loss (mean over the rows with a label in [0, V)), loss per row, their count, dh or undefined}.
 std::vector<Tensor> lm_head_ce_pieces(Tensor h, c10::optional<Tensor> W, c10::optional<Tensor> codes,
@@ -916,6 +932,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("mx4_dequantize", &mx4_dequantize);
   m.def("mx4_embed", &mx4_embed);
   m.def("mx4_linear", &mx4_linear);
+  m.def("mx4_linear_grad", &mx4_linear_grad, "mx4_linear as an autograd node, gradient to x");
   m.def("mx4_dgrad", &mx4_dgrad);
   m.def("lm_head_ce_pieces", &lm_head_ce_pieces);
   m.def("lm_head_ce_pieces_width", &mft::lm_head_ce_pieces_width, "default columns of a vocabulary piece for M rows");

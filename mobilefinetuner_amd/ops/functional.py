@@ -645,8 +645,11 @@ class _MX4Linear(Function):
 def mx4_linear(x, w, b=None):
     """y = x W^T + b for an MX4Weight W [out, in]: x bf16 [.., in] of one row or many -> [.., out].  The
     gradient goes to x (and to b); W is frozen."""
-    if torch.is_grad_enabled() and (x.requires_grad or _needs(b)):
-        return _MX4Linear.apply(x, w, b)
+    if torch.is_grad_enabled():
+        if _needs(b):
+            return _MX4Linear.apply(x, w, b)
+        if x.requires_grad:
+            return native().mx4_linear_grad(x, w.codes, w.scales, cw(b))
     return native().mx4_linear(x, w.codes, w.scales, cw(b))
 
 

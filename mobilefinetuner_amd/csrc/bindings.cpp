@@ -413,7 +413,9 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   mft::Mx4LinearArgs a{};
   a.codes = u8p(codes); a.scales = u8p(scales);
   a.x = bp(x2); a.ldx = x2.stride(0);
-  a.bias = optp<bf16_t>(bias);
+  Tensor b;
+  if (bias.has_value() && bias->defined()) b = reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 ? bias->clone() : *bias;
+  a.bias = b.defined() ? bp(b) : nullptr;
   a.y = bp(y); a.ldy = out;
   a.M = (int)x2.size(0); a.N = (int)N; a.K = K;
   if (!dgrad && mft::mx4_few_rows(a.M, a.N, a.K)) {

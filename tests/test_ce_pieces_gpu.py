@@ -287,3 +287,41 @@ def test_memory_after_the_vocabulary_is_not_used(m, k, v, piece):
     loss, dh = _check(h, buf[:v], wd, labels, v, piece)
     again, dh2 = _run(h, buf, labels, v, piece)
     assert torch.equal(loss, again) and torch.equal(dh, dh2)
+
+
+@pytest.mark.parametrize("table", ["bf16", "mx4"])
+def test_piece_past_32_bits(table):
+    """16,640 rows x 262,144 columns in one piece: 4.36e9 exponentials.  The last rows against the formula."""
+    m, k, v, last = 16640, 128, 262144, 40
+    h, w, wd, labels = _case(m, k, v, table, seed=12)
+    x = h.requires_grad_(True)
+    loss = _fx().lm_head_cross_entropy_pieces(x, w, labels, v, v)
+    (dh,) = torch.autograd.grad(loss, x)
+    n, n_last = int((labels >= 0).sum()), int((labels[-last:] >= 0).sum())
+    _, want, room, _ = _exact(h.detach()[-last:], wd, labels[-last:])
+    over = (dh[-last:].double() - want * (n_last / n)).abs() - room * (n_last / n)
+    assert over.max().item() <= 0, over.max().item()
+    assert dh[labels < 0].abs().max().item() == 0.0
+
+
+def test_two_streams_at_once():
+    cases = [_case(m, 128, 3000, "mx4", seed=m) for m in (30, 700)]
+    want = [_run(h, w, labels, 3000, 512) for h, w, _, labels in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_run(cases[i][0], cases[i][1], cases[i][3], 3000, 512))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+def test_backward_twice():
+    h, w, _, labels = _case(90, 128, 1000, "mx4")
+    x = h.requires_grad_(True)
+    loss = _fx().lm_head_cross_entropy_pieces(x, w, labels, 1000)
+    (a,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (b,) = torch.autograd.grad(loss, x)
+    assert torch.equal(a, b)

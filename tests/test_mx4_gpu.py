@@ -307,3 +307,93 @@ def test_refusals():
     p = torch.zeros(2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
     with pytest.raises(RuntimeError, match="position table"):
         Fx.mx4_embedding(torch.zeros(1, 2, device="cuda", dtype=torch.long), w4, p)
+
+
+# ---------------------------------------------------------------- every tile shape, split and the bf16 copy
+SHAPES = [(7295, 1056, 128), (8664, 199, 128), (9432, 65, 1824), (8352, 395, 128), (8800, 386, 3456), (16, 16, 1344), (699, 16, 1504),
+          (147, 5450, 128), (18, 2706, 2592), (1438, 16, 2016), (33, 2815, 2720), (570, 6695, 160), (261, 7211, 3712),
+          (6788, 192, 1184), (599, 16, 3456), (65, 2470, 3808), (9817, 16, 1280), (6995, 3264, 544), (17, 717, 128),
+          (16, 1530, 1472), (33, 3015, 352), (34, 1067, 2720), (5415, 6592, 160), (4099, 2304, 768)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_large_and_ragged_products(m, n, k):
+    w4 = _weight(n, k, seed=m)
+    x = torch.randn(m, k, device="cuda", generator=_gen(n)).bfloat16().requires_grad_(True)
+    b = torch.randn(n, device="cuda", generator=_gen(k)).bfloat16()
+    dy = torch.randn(m, n, device="cuda", generator=_gen(k + 1)).bfloat16()
+    y = _fx().mx4_linear(x, w4, b)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    v, xd, dd = ref.values(w4.codes, w4.scales).cuda(), x.detach().double(), dy.double()
+    _check(y.detach(), xd @ v.t() + b.double(), xd.abs() @ v.abs().t() + b.double().abs(), k)
+    _check(dx, dd @ v, dd.abs() @ v.abs(), n)
+
+
+@pytest.mark.parametrize("m", [2, 40, 4100])
+def test_bias_at_any_address(m):
+    """A contiguous bias that starts inside a 16-byte word."""
+    n, k = 13824 if m == 2 else 1024, 512
+    w4 = _weight(n, k)
+    x = torch.randn(m, k, device="cuda", generator=_gen(1)).bfloat16()
+    long = torch.randn(n + 3, device="cuda", generator=_gen(2)).bfloat16()
+    for o in (1, 2, 3):
+        assert torch.equal(_fx().mx4_linear(x, w4, long[o:o + n]), _fx().mx4_linear(x, w4, long[o:o + n].clone()))
+
+
+def test_one_weight_twice_in_a_graph():
+    """A weight used by two products of one graph, and a graph walked twice: the gradients add, nothing is kept."""
+    Fx = _fx()
+    w4 = _weight(96, 96)
+    x = torch.randn(70, 96, device="cuda", generator=_gen(3)).bfloat16().requires_grad_(True)
+    dy = torch.randn(70, 96, device="cuda", generator=_gen(4)).bfloat16()
+    y = Fx.mx4_linear(Fx.mx4_linear(x, w4), w4)
+    (a,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    (b,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    assert torch.equal(a, b)
+    (c,) = torch.autograd.grad(y, x, dy + dy)
+    assert torch.equal(c, a + a)
+
+
+def test_training_on_two_streams_at_once():
+    Fx = _fx()
+    w4 = _weight(2304, 768)
+    g = _gen(5)
+    xs = [torch.randn(m, 768, device="cuda", generator=g).bfloat16().requires_grad_(True) for m in (100, 1500)]
+    dys = [torch.randn(x.shape[0], 2304, device="cuda", generator=g).bfloat16() for x in xs]
+    want = [torch.autograd.grad(Fx.mx4_linear(x, w4), x, dy)[0] for x, dy in zip(xs, dys)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(torch.autograd.grad(Fx.mx4_linear(xs[i], w4), xs[i], dys[i])[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(d, want[i]) for d in got[i])
+
+
+def test_codes_past_4_gib():
+    """2,097,180 x 4,128: codes of 4.3 GB.  Its last rows give what they give as a weight of their own."""
+    Fx = _fx()
+    n, k, last = 2097180, 4128, 60
+    codes = torch.zeros(n, k // 2, device="cuda", dtype=torch.uint8)
+    scales = torch.full((n, k // 32), 127, device="cuda", dtype=torch.uint8)
+    codes[-last:] = torch.randint(0, 256, (last, k // 2), device="cuda", generator=_gen(6)).to(torch.uint8)
+    scales[-last:] = torch.randint(118, 122, (last, k // 32), device="cuda", generator=_gen(7)).to(torch.uint8)
+    w4, end = Fx.MX4Weight(codes, scales), Fx.MX4Weight(codes[-last:].clone(), scales[-last:].clone())
+    v = ref.values(end.codes, end.scales).cuda()
+    for m in (1, 8, 40):
+        x = torch.randn(m, k, device="cuda", generator=_gen(m)).bfloat16().requires_grad_(True)
+        y = Fx.mx4_linear(x, w4)
+        xd = x.detach().double()
+        _check(y.detach()[:, -last:], xd @ v.t(), xd.abs() @ v.abs().t(), k)
+        assert y.detach()[:, :-last].abs().max().item() == 0.0
+        dy = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+        dy[:, -last:] = torch.randn(m, last, device="cuda", generator=_gen(m + 1)).bfloat16()
+        (dx,) = torch.autograd.grad(y, x, dy)
+        d = dy[:, -last:].double()
+        _check(dx, d @ v, d.abs() @ v.abs(), last)
+    ids = torch.tensor([[n - 1, n - last, 0]], device="cuda")
+    out = Fx.mx4_embedding(ids, w4)
+    assert torch.equal(out[0], v[-1].bfloat16()) and torch.equal(out[1], v[0].bfloat16()) and out[2].abs().max().item() == 0.0
+    assert torch.equal(Fx.mx4_quantize(end.dequantize()).dequantize(), end.dequantize())

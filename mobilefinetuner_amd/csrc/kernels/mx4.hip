@@ -22,6 +22,8 @@ namespace {
 // byte is e + 127 - 2, one more when f > 1.75.  |w| 2^(127 - byte) is then at most 7; above 6 it saturates,
 // off by at most 1 -- half a step at that size, as everywhere on the grid.  Nearest code, ties to even.
 // A group that holds an infinity or a NaN gets byte 255 (it reads as NaN) and codes 0.
+// Bound by memory, read once in 16- and 32-B loads, a lane's 8 columns its whole state: 262144 x 640 fp32 135 us
+// (5.6 TB/s), 262144 x 1152 bf16 130 us (5.9 TB/s); 2304 x 768 is one launch, 5 us.
 template <bool F32>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restrict__ w, uint32_t* __restrict__ codes,
                                                            uint8_t* __restrict__ scales, long n8) {
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* __restric
 
 // ------------------------------------------------------------------ dequantise, embedding
 // out[r, 0 : K] = W[n0 + r] for r < rows; columns K .. kpad - 1 and rows past N are zeros (the padded
-// operand of a GEMM).  One lane per 8 columns: 4 B of codes in, 16 B out.
+// operand of a GEMM).  One lane per 8 columns: 4 B of codes in, 16 B out.  Bound by the writes: 262144 x 640 87 us (4.9 TB/s).
 __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint32_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ scales, long n0, long N, int K,
                                                           bf16_t* __restrict__ out, long ldo, long rows, int kpad) {
@@ -70,7 +72,8 @@ __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint32_t* __rest
   *reinterpret_cast<bf16x8_t*>(out + r * ldo + c8 * 8) = v;
 }
 
-// out[m] = W[ids[m]] * scale (+ wpe[m % S]), rounded once.  An id outside [0, N) gives a row of NaN.
+// out[m] = W[ids[m]] * scale (+ wpe[m % S]), rounded once.  An id outside [0, N) gives a row of NaN.  Bound by the writes
+// and, for ids all over the table, by rows of a few hundred bytes: 65536 x 640 20 us with the ids of text, 24 us at random.
 __global__ __launch_bounds__(256) void mx4_embed_kernel(const int64_t* __restrict__ ids, const uint32_t* __restrict__ codes,
                                                         const uint8_t* __restrict__ scales, long N, int K,
                                                         const bf16_t* __restrict__ wpe, bf16_t* __restrict__ out, long M,
@@ -101,6 +104,7 @@ __global__ __launch_bounds__(256) void mx4_embed_kernel(const int64_t* __restric
 // operands of four 16x16x32 MFMAs; step t multiplies columns 32 (l >> 4) + 8 t + j, so x is read with the
 // same permutation.  Nothing is staged: codes and x go from memory into the operands, the loads of U such
 // chunks in flight together.  S waves of a workgroup share a column tile and split K; they meet in LDS.
+// Bound by a launch and one or two rounds of loads: 1 x 2304 x 768 3.2 us, 16 rows 4.2 us, 64 rows 5.5 us.
 template <int MT, int TN, int S, int U>
 __global__ __launch_bounds__(64 * (S > 4 ? S : 4)) void mx4_rows_kernel(Mx4LinearArgs g) {
   constexpr int NW = S > 4 ? S : 4, TPB = NW / S;  // waves, column tiles (of TN * 16) per workgroup

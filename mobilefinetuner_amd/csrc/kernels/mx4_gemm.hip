@@ -10,6 +10,11 @@
 //        back transposed (ds_read_b64_tr_b4: a lane gets 16 rows of its column); every row has its own scale, so a
 //        byte (two rows) is converted under both scales and the halves are picked.
 // The reduction may be split over workgroups (few tiles): fp32 slabs, summed in split order by mx4_join.
+// Small products are bound by a step's latency (loads to LDS, barrier, products): 512 x 2304 x 768 y 9.9 us, dx 15.6 us;
+// large ones by the conversions, which share the vector unit's issue with the MFMAs: 32768 x 13824 x 1152 y 895 us
+// (1166 TF), dx 999 us (1045 TF).  Through a bf16 copy and gemm4 those take 747 us (1397 TF) and 822 us (1270 TF), which
+// pays from about 2e10 multiplications on (8192 x 13824 x 1152 212 / 264 us against 231 / 302 us; 1999 x 6400 x 1600 y 49
+// against 52 us; 8192 x 2304 x 768 by tiles, 39 / 42 us): mx4_plan models both.
 #include "common.h"
 #include "kernels.h"
 #include "mx4.h"

@@ -6,11 +6,11 @@
 // operands in registers, so a step's LDS traffic is the activation's alone.
 //   y  = x W^T: the reduction runs along the codes.  A lane loads 16 B -- one scale group -- of its column's row of
 //        W, 128 columns of K a step, straight from memory.
-//   dx = dy W: the reduction runs across the rows of W, 64 a step.  Their codes go through LDS as they are and come
+//   dx = dy W: the reduction runs across the rows of W, 64 or 128 a step.  Their codes go through LDS as they are and come
 //        back transposed (ds_read_b64_tr_b4: a lane gets 16 rows of its column); every row has its own scale, so a
 //        byte (two rows) is converted under both scales and the halves are picked.
 // The reduction may be split over workgroups (few tiles): fp32 slabs, summed in split order by mx4_join.
-// Small products are bound by a step's latency (loads to LDS, barrier, products): 512 x 2304 x 768 y 9.9 us, dx 15.6 us;
+// Small products are bound by a step's latency (loads to LDS, barrier, products): 512 x 2304 x 768 y 9.9 us, dx 14.9 us;
 // large ones by the conversions, which share the vector unit's issue with the MFMAs: 32768 x 13824 x 1152 y 895 us
 // (1166 TF), dx 999 us (1045 TF).  Through a bf16 copy and gemm4 those take 747 us (1397 TF) and 822 us (1270 TF), which
 // pays from about 2e10 multiplications on (8192 x 13824 x 1152 212 / 264 us against 231 / 302 us; 1999 x 6400 x 1600 y 49
@@ -42,9 +42,19 @@ __device__ __forceinline__ void arrive() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// 64-row blocks of W in a dx step: two in the small tiles, whose steps are bound by latency (2048 x 2304 x 768 22.7 us, with
+// one 26.7 us; 128 x 128 tiles lose by it: 70.7 against 68.5 us on 1999 x 6400 x 1600)
+template <int BM, int TN>
+constexpr int kBlocks = BM * TN <= 128 ? 2 : 1;
+
+// reduction length of a step
+template <int BM, int TN, bool DG>
+constexpr int kStep = DG ? 64 * kBlocks<BM, TN> : 128;
+
 template <int BM, int TN, bool DG>
 constexpr int lds_bytes() {
-  return 2 * (DG ? BM * 128 + 64 * (32 * TN + 16) + 64 * 4 * 2 * TN : BM * 256);
+  constexpr int st = kStep<BM, TN, DG>;
+  return 2 * (BM * st * 2 + (DG ? st * (32 * TN + 16) + st * 4 * 2 * TN : 0));
 }
 
 // Scale bytes travel as unaligned 32-bit words of four neighbouring groups, the byte taken at its use: a byte kept in
@@ -69,7 +79,7 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
   const int split = bid / (tn * tm), tile = bid - split * (tn * tm);
   const int grp0 = tile / (8 * tn) * 8, gsz = min(8, tm - grp0), in_grp = tile - grp0 * tn;
   const int m0 = (grp0 + in_grp % gsz) * BM, c0 = in_grp / gsz * BN;
-  constexpr int STEP = DG ? 64 : 128;
+  constexpr int STEP = kStep<BM, TN, DG>, H = kBlocks<BM, TN>;
   const int steps = (red + STEP - 1) / STEP, per = (steps + splits - 1) / splits;
   const int s0 = split * per, s1 = min(s0 + per, steps);
 
@@ -79,19 +89,20 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = zero4();
 
-  // ---- the activation tile: [BM][STEP] bf16 in 16-B chunks.  Lane group kq of an operand read takes chunk
-  // kq * (CPR / 4) + t of 16 rows; it is stored at slot (4 t + kq) ^ swz(row).  The hardware serves a 16-B read 16
+  // ---- the activation tile: [BM][STEP] bf16 in 16-B chunks.  Lane group kq of an operand read takes chunk 4 kq + t of
+  // 16 rows (dx: 8 (t / 2) + 2 kq + t % 2, as the transposed codes come); it is stored at slot (4 t + kq) ^ swz(row).  The hardware serves a 16-B read 16
   // lanes at a time, rows 0-3 and 12-15 of one lane group with rows 4-11 of the next: with kq in the slot's low bits
   // those 16 fall into different banks (in the chunk's own order they met in pairs: half of all LDS cycles).
   // Rows past M repeat the last one (never stored); chunks past the reduction's end repeat the last one and are
   // zeroed in LDS by tail() before use.
   constexpr int CPR = STEP / 8, ALOADS = BM * CPR / 256;  // chunks per row, loads per thread
   const bf16_t* abase = g.x + (long)m0 * g.ldx;
-  auto swz = [](int row) { return DG ? (row >> 1) & 7 : row & 15; };
+  auto swz = [](int row) { return CPR == 8 ? (row >> 1) & 7 : row & 15; };
   const int chunks = DG ? (red + 7) / 8 : red / 8;  // chunks that exist in a row
   // thread tid loads slot tid % CPR of rows tid / CPR + t * 256 / CPR, all with the same swizzle
   constexpr int RPL = 256 / CPR;
-  const int arow = tid / CPR, asl = (tid % CPR) ^ swz(arow), achk = (asl & 3) * (CPR / 4) + (asl >> 2);
+  const int arow = tid / CPR, asl = (tid % CPR) ^ swz(arow);
+  const int achk = DG ? (asl >> 3) * 8 + (asl & 3) * 2 + ((asl >> 2) & 1) : (asl & 3) * 4 + (asl >> 2);
   const int mlast = g.M - 1 - m0, lda = (int)g.ldx;
   auto abuf = [&](int buf) { return reinterpret_cast<bf16_t*>(smem) + buf * (BM * STEP); };
   auto load_a = [&](int buf, int s) {
@@ -189,33 +200,41 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
     constexpr int CLD = BN / 2 + 16;           // bytes of a staged code row: 16 rows of 8-B reads hit different banks
     constexpr int CBT = BN / 8;                // code bytes per thread: 8, 16 or 32
     constexpr int NG = BN / 32;                // scale groups of a code row: 2, 4 or 8; its four threads share them out
-    char* cbase = smem + 2 * BM * 128;
-    float* sbase = reinterpret_cast<float*>(cbase + 2 * 64 * CLD);
+    char* cbase = smem + 2 * BM * STEP * 2;
+    float* sbase = reinterpret_cast<float*>(cbase + 2 * STEP * CLD);
     const int crow = tid >> 2, cseg = (tid & 3) * CBT;
     const int ng = g.K / 32;
-    uint2 q[CBT / 8];  // the next step's, on their way to LDS
-    uint32_t sw;
+    uint2 q[H][CBT / 8];  // the next step's, on their way to LDS
+    uint32_t sw[H];
     const int sgrp = NG == 8 ? (tid & 3) * 2 : (tid & 3) % NG;  // this thread's first group of the row
     const int sfirst = NARROW ? c0 / 32 + sgrp : min(c0 / 32 + (sgrp & ~3), g.K / 32 - 4);
     auto load_c = [&](int s) {
-      const uint8_t* p = g.codes + (long)min(s * 64 + crow, g.N - 1) * (g.K / 2);
 #pragma unroll
-      for (int e = 0; e < CBT / 8; ++e) q[e] = *reinterpret_cast<const uint2*>(p + min(c0 / 2 + cseg + e * 8, g.K / 2 - 8));
-      const uint8_t* sp = g.scales + (long)min(s * 64 + crow, g.N - 1) * ng;
-      if constexpr (NARROW) sw = sp[min(sfirst, ng - 1)];
-      else sw = load_u32(sp + sfirst);
+      for (int hb = 0; hb < H; ++hb) {
+        const long n = min(s * STEP + hb * 64 + crow, g.N - 1);
+        const uint8_t* p = g.codes + n * (g.K / 2);
+#pragma unroll
+        for (int e = 0; e < CBT / 8; ++e) q[hb][e] = *reinterpret_cast<const uint2*>(p + min(c0 / 2 + cseg + e * 8, g.K / 2 - 8));
+        const uint8_t* sp = g.scales + n * ng;
+        if constexpr (NARROW) sw[hb] = sp[min(sfirst, ng - 1)];
+        else sw[hb] = load_u32(sp + sfirst);
+      }
     };
     // rows past N become zeros; columns past K are never stored
     auto put_c = [&](int buf, int s) {
-      const bool in = s * 64 + crow < g.N;
-      char* cb = cbase + buf * 64 * CLD;
 #pragma unroll
-      for (int e = 0; e < CBT / 8; ++e) *reinterpret_cast<uint2*>(cb + crow * CLD + cseg + e * 8) = in ? q[e] : uint2{0, 0};
-      float* sb = sbase + buf * 64 * NG + crow;
+      for (int hb = 0; hb < H; ++hb) {
+        const int row = hb * 64 + crow;
+        const bool in = s * STEP + row < g.N;
+        char* cb = cbase + buf * STEP * CLD + row * CLD + cseg;
 #pragma unroll
-      for (int e = 0; e < (NG == 8 ? 2 : 1); ++e) {
-        const uint32_t byte = NARROW ? sw : sw >> ((c0 / 32 + sgrp + e - sfirst) * 8 & 31) & 255u;
-        sb[(sgrp + e) * 64] = mx4_scale(in ? byte : 127u);
+        for (int e = 0; e < CBT / 8; ++e) *reinterpret_cast<uint2*>(cb + e * 8) = in ? q[hb][e] : uint2{0, 0};
+        float* sb = sbase + buf * STEP * NG + row;
+#pragma unroll
+        for (int e = 0; e < (NG == 8 ? 2 : 1); ++e) {
+          const uint32_t byte = NARROW ? sw[hb] : sw[hb] >> ((c0 / 32 + sgrp + e - sfirst) * 8 & 31) & 255u;
+          sb[(sgrp + e) * STEP] = mx4_scale(in ? byte : 127u);
+        }
       }
     };
     if (s0 < s1) {
@@ -227,20 +246,22 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
       const int buf = (s - s0) & 1;
       arrive();
       // (before the next loads go out: the compiler makes a transposed read wait for every load to LDS in flight)
-      i32x2_t raw[TN];
+      i32x2_t raw[H][TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-        raw[j] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)(
-            cbase + buf * 64 * CLD + lane * CLD + (w * TN + j) * 8));
+      for (int hb = 0; hb < H; ++hb)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          raw[hb][j] = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)(
+              cbase + (buf * STEP + hb * 64 + lane) * CLD + (w * TN + j) * 8));
       tail(buf, s);
       load_c(min(s + 1, s1 - 1));
       load_a(buf ^ 1, min(s + 1, s1 - 1));
-      const float* sl = sbase + buf * 64 * NG + kq * 16;
-      products(buf, [&](bf16x8_t (&b)[TN], int h) {  // rows 16 kq + 8 h + 0 .. 7 of the step
+      const float* sl = sbase + buf * STEP * NG + kq * 16;
+      products(buf, [&](bf16x8_t (&b)[TN], int t) {  // rows 64 (t / 2) + 16 kq + 8 (t % 2) + 0 .. 7 of the step
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          const float* p = sl + ((w * TN + j) >> 1) * 64 + h * 8;
-          b[j] = mx4_cvt8((uint32_t)raw[j][h], *reinterpret_cast<const f32x4_t*>(p), *reinterpret_cast<const f32x4_t*>(p + 4));
+          const float* p = sl + ((w * TN + j) >> 1) * STEP + (t >> 1) * 64 + (t & 1) * 8;
+          b[j] = mx4_cvt8((uint32_t)raw[t >> 1][j][t & 1], *reinterpret_cast<const f32x4_t*>(p), *reinterpret_cast<const f32x4_t*>(p + 4));
         }
       });
       put_c(buf ^ 1, s + 1);
@@ -395,7 +416,7 @@ namespace {
 // Modelled time of a tile shape, in us: a0 + steps of a workgroup x max(lat, workgroups per CU x thr) + workgroups per
 // CU x fix (+ the join: j0 + slab bytes at jb TB/s).  lat: a step alone on its CU, bound by a load's latency; thr: a step's
 // share of a busy CU; fix: a workgroup's start and stores.  Fitted to 320 products (1 to 16,384 rows, 12 weights, every
-// shape and split): the shape picked costs 3 % (y) and 6 % (dx) over the best one on average, at worst 22 % and 42 %.
+// shape and split): the shape picked costs 3 % (y) and 2 % (dx) over the best one on average, at worst 22 % and 17 %.
 struct TileCost {
   int bm, tn;
   float lat, thr, fix;
@@ -403,26 +424,26 @@ struct TileCost {
 constexpr TileCost kCostY[] = {{128, 4, 2.07f, 1.32f, 4.4f}, {128, 2, 1.27f, 0.86f, 2.5f}, {64, 4, 1.37f, 0.90f, 2.8f},
                                {64, 2, 0.87f, 0.55f, 1.7f},  {64, 1, 0.64f, 0.43f, 1.2f},  {32, 2, 0.66f, 0.41f, 1.3f},
                                {32, 1, 0.47f, 0.30f, 0.85f}, {16, 1, 0.45f, 0.26f, 0.8f}};
-constexpr TileCost kCostDx[] = {{128, 4, 1.28f, 0.78f, 3.5f}, {128, 2, 0.81f, 0.48f, 1.9f}, {64, 4, 0.96f, 0.54f, 1.9f},
-                                {64, 2, 0.66f, 0.36f, 1.2f},  {64, 1, 0.55f, 0.29f, 0.78f}, {32, 2, 0.56f, 0.30f, 0.81f},
-                                {32, 1, 0.49f, 0.20f, 0.61f}};
+constexpr TileCost kCostDx[] = {{128, 4, 1.32f, 0.81f, 2.1f}, {128, 2, 0.83f, 0.49f, 1.4f}, {64, 4, 1.01f, 0.56f, 1.5f},
+                                {64, 2, 1.02f, 0.74f, 0.90f}, {64, 1, 0.85f, 0.58f, 0.47f}, {32, 2, 0.81f, 0.57f, 0.38f},
+                                {32, 1, 0.71f, 0.43f, 0.30f}};
 
 }  // namespace
 
 Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits, bool dense) {
   if (K < 128) return Mx4Plan{64, 2, 1, 0};  // the narrow kernel
   const long cols = dgrad ? K : N, red = dgrad ? N : K;
-  const long steps = dgrad ? (red + 63) / 64 : (red + 127) / 128;
   Mx4Plan best{};
   double best_t = 1e30;
   auto consider = [&](const TileCost& c) {
     if (M <= c.bm / 2 && c.bm > 32) return;  // (32 rows: the smallest dx tile)
     const long tiles = (M + c.bm - 1L) / c.bm * ((cols + 64 * c.tn - 1) / (64 * c.tn));
+    const long step = dgrad && c.bm * c.tn > 128 ? 64 : 128, steps = (red + step - 1) / step;
     for (int s = 1; s <= max_splits; s += s < 4 ? 1 : s < 8 ? 2 : s < 16 ? 4 : 8) {
       if (s > 1 && (steps / s < 2 || tiles * s > 2048)) break;
       const double n = (double)((tiles * s + 255) / 256), per = (double)((steps + s - 1) / s);
-      double t = (dgrad ? 2.6 : 3.0) + per * std::max((double)c.lat, n * c.thr) + n * c.fix;
-      if (s > 1) t += (dgrad ? 4.2 : 3.2) + (double)s * M * cols * 4 / 3.2e6;
+      double t = (dgrad ? 3.6 : 3.0) + per * std::max((double)c.lat, n * c.thr) + n * c.fix;
+      if (s > 1) t += (dgrad ? 3.4 : 3.2) + (double)s * M * cols * 4 / (dgrad ? 2.8e6 : 3.2e6);
       if (t < best_t) best_t = t, best = Mx4Plan{c.bm, c.tn, s, 0};
     }
   };

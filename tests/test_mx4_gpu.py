@@ -313,7 +313,8 @@ def test_refusals():
 SHAPES = [(7295, 1056, 128), (8664, 199, 128), (9432, 65, 1824), (8352, 395, 128), (8800, 386, 3456), (16, 16, 1344), (699, 16, 1504),
           (147, 5450, 128), (18, 2706, 2592), (1438, 16, 2016), (33, 2815, 2720), (570, 6695, 160), (261, 7211, 3712),
           (6788, 192, 1184), (599, 16, 3456), (65, 2470, 3808), (9817, 16, 1280), (6995, 3264, 544), (17, 717, 128),
-          (16, 1530, 1472), (33, 3015, 352), (34, 1067, 2720), (5415, 6592, 160), (4099, 2304, 768)]
+          (16, 1530, 1472), (33, 3015, 352), (34, 1067, 2720), (5415, 6592, 160), (4099, 2304, 768), (4190, 16, 160),
+          (2085, 5696, 160), (8236, 192, 1536), (5402, 22, 704)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

@@ -43,7 +43,7 @@ __device__ __forceinline__ void arrive() {
 }
 
 // 64-row blocks of W in a dx step: two in the small tiles, whose steps are bound by latency (2048 x 2304 x 768 22.7 us, with
-// one 26.7 us; 128 x 128 tiles lose by it: 70.7 against 68.5 us on 1999 x 6400 x 1600)
+// one 26.7 us; 128 x 128 tiles lose by it: 70.7 against 68.5 us on 1999 x 6400 x 1600).  256 columns a step of y gain nothing.
 template <int BM, int TN>
 constexpr int kBlocks = BM * TN <= 128 ? 2 : 1;
 
@@ -90,9 +90,10 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
     for (int j = 0; j < TN; ++j) acc[i][j] = zero4();
 
   // ---- the activation tile: [BM][STEP] bf16 in 16-B chunks.  Lane group kq of an operand read takes chunk 4 kq + t of
-  // 16 rows (dx: 8 (t / 2) + 2 kq + t % 2, as the transposed codes come); it is stored at slot (4 t + kq) ^ swz(row).  The hardware serves a 16-B read 16
-  // lanes at a time, rows 0-3 and 12-15 of one lane group with rows 4-11 of the next: with kq in the slot's low bits
-  // those 16 fall into different banks (in the chunk's own order they met in pairs: half of all LDS cycles).
+  // 16 rows (dx: 8 (t / 2) + 2 kq + t % 2, as the transposed codes come); it is stored at slot (4 t + kq) ^ swz(row).
+  // The hardware serves a 16-B read 16 lanes at a time, rows 0-3 and 12-15 of one lane group with rows 4-11 of the
+  // next: with kq in the slot's low bits those 16 fall into different banks (in the chunk's own order they met in
+  // pairs: half of all LDS cycles).
   // Rows past M repeat the last one (never stored); chunks past the reduction's end repeat the last one and are
   // zeroed in LDS by tail() before use.
   constexpr int CPR = STEP / 8, ALOADS = BM * CPR / 256;  // chunks per row, loads per thread

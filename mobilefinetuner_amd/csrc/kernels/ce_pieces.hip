@@ -318,8 +318,9 @@ struct Plan {
 };
 
 // Rows up to which a 4-bit table is multiplied as it is, loss and gradient in us there / through the bf16 workspace:
-// 262144 x 640 1 row 115 / 240, 64 rows 167 / 250, 256 rows 469 / 474; 262144 x 1152 256 rows 540 / 710; 50257 x 768 256 rows 138 / 143.
-constexpr int kFewRows = 256;
+// 262144 x 640 1 row 83 / 349, 64 rows 138 / 351, 200 rows 341 / 380, 256 rows 414 / 381; 262144 x 1152 200 rows 449 / 560,
+// 256 rows 522 / 566; 50257 x 768 64 rows 61 / 105, 200 rows 119 / 115, 256 rows 130 / 116.
+constexpr int kFewRows = 192;
 
 int up64(int x) { return (x + 63) / 64 * 64; }
 
@@ -339,8 +340,8 @@ int dgrad_splits(int M, int K, int w) {
   return best;
 }
 
-// the slabs of a few-rows gradient product over w columns of the vocabulary
-Mx4Plan few_plan(const CePiecesArgs& a, int w) { return mx4_plan(a.M, w, a.K, true, up64(w), 32, false); }
+// the slabs of a few-rows gradient product over w columns of the vocabulary (64 splits, with 32: 262144 x 640 1 row 97 us)
+Mx4Plan few_plan(const CePiecesArgs& a, int w) { return mx4_plan(a.M, w, a.K, true, up64(w), 64, false); }
 
 Plan make_plan(const CePiecesArgs& a) {
   Plan p{};

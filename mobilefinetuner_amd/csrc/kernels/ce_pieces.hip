@@ -331,7 +331,7 @@ int dgrad_splits(int M, int K, int w) {
   const int nk = (w + 63) / 64, tiles = ((M + 255) / 256) * ((K + 255) / 256), cus = num_cus();
   int best = 1;
   double best_t = 1e30;
-  for (int sp = 1; sp <= 64 && (sp == 1 || nk / sp >= 16); ++sp) {
+  for (int sp = 1; sp <= 64 && sp <= nk; ++sp) {
     const int kps = (nk + sp - 1) / sp;
     if (sp > 1 && (kps % 4 || (long)(sp - 1) * kps >= nk)) continue;
     const double t = (tiles * sp + cus - 1) / cus * (5 + 2.1 * kps) + (sp > 1 ? (double)sp * M * K * 8 / 4.5e6 : 0);

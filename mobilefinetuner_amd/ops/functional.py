@@ -1154,29 +1154,6 @@ def lm_head_cross_entropy(h, w, labels, vocab_size, chunk=None, w_grad_scale=1.0
     return _LMHeadCE.apply(h, w, labels, int(vocab_size), int(chunk), float(w_grad_scale))
 
 
-class _LMHeadCEPieces(Function):
-    """The loss and -- in the same sweep over the vocabulary -- dh (kernels/ce_pieces.hip); the backward pass
-    multiplies dh by the loss's gradient."""
-
-    @staticmethod
-    def forward(ctx, h, w, labels, V, piece):
-        loss, dh = _ce_pieces(h, w, labels, V, piece, ctx.needs_input_grad[0])
-        ctx.save_for_backward(dh)
-        return loss
-
-    @staticmethod
-    def backward(ctx, gout):
-        (dh,) = ctx.saved_tensors
-        return native().scale_bf16(dh, gout.float().reshape(1), 1.0), None, None, None, None
-
-
-def _ce_pieces(h, w, labels, V, piece, grad):
-    mx = isinstance(w, MX4Weight)
-    loss, _, _, dh = native().lm_head_ce_pieces(h, None if mx else cw(w), w.codes if mx else None, w.scales if mx else None,
-                                                labels.reshape(-1), V, piece, grad)
-    return loss, dh
-
-
 @_device_op
 def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
     """Mean token NLL of logits = h W^T over the rows whose label lies in [0, vocab_size) (others, -100 among
@@ -1187,10 +1164,12 @@ def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
     an MX4Weight; the gradient goes to h.  A trainable W is lm_head_cross_entropy's."""
     if _needs(w):
         raise RuntimeError("lm_head_cross_entropy_pieces: W is frozen here; lm_head_cross_entropy trains it")
-    piece = int(piece or 0)
+    mx = isinstance(w, MX4Weight)
+    args = (h, None if mx else cw(w), w.codes if mx else None, w.scales if mx else None, labels.reshape(-1), int(vocab_size),
+            int(piece or 0))
     if torch.is_grad_enabled() and h.requires_grad:
-        return _LMHeadCEPieces.apply(h, w, labels, int(vocab_size), piece)
-    return _ce_pieces(h, w, labels, int(vocab_size), piece, False)[0]
+        return native().lm_head_ce_pieces_grad(*args)  # dh in the same sweep; the backward pass scales it
+    return native().lm_head_ce_pieces(*args, False)[0]
 
 
 @_device_op

@@ -380,14 +380,15 @@ Tensor mx4_embed(Tensor ids, Tensor codes, Tensor scales, c10::optional<Tensor> 
   return out;
 }
 
-// the [rows, width] operand of an mx4 product: itself where 16-byte loads may walk it, else a copy; `zpad`:
-// columns past the width up to the next multiple of 8 are read and have to be zeros
-Tensor mx4_operand(const Tensor& x, long width, bool zpad) {
-  Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, width});
-  if (rows16(x2) && !(zpad && width % 8)) return x2;
-  auto c = (zpad && width % 8) ? torch::zeros({x2.size(0), (width + 7) / 8 * 8}, x2.options())
-                               : torch::empty({x2.size(0), (width + 7) / 8 * 8}, x2.options());
-  c.narrow(1, 0, width).copy_(x2);
+// the [rows, width] operand of an mx4 product: itself where 16-byte loads may walk it, else a copy; a width that is no
+// multiple of 8 is copied with zeros up to the next multiple of 64
+Tensor mx4_operand(const Tensor& x, long width) {
+  const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, width});
+  if (rows16(x2) && width % 8 == 0) return x2;
+  const long wide = width % 8 ? (width + 63) / 64 * 64 : width;
+  auto c = torch::empty({x2.size(0), wide}, x2.options());
+  const Tensor src = x2.stride(1) == 1 ? x2 : x2.contiguous();
+  mft::mx4_pad_rows(bp(src), src.stride(0), src.size(0), (int)width, bp(c), (int)wide, stream());
   return c;
 }
 
@@ -408,7 +409,7 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   auto y = torch::empty(sizes, x.options());
   if (y.numel() == 0) return y;
   if (in == 0) return y.zero_();
-  const Tensor x2 = mx4_operand(x, in, dgrad);
+  const Tensor x2 = mx4_operand(x, in);
   TORCH_CHECK(x2.size(0) <= 0x3fffffff, what, ": too many rows");
   mft::Mx4LinearArgs a{};
   a.codes = u8p(codes); a.scales = u8p(scales);
@@ -422,10 +423,10 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
     mft::mx4_rows(a, stream());
     return y;
   }
-  const auto plan = mft::mx4_plan(a.M, a.N, a.K, dgrad, a.ldx);
+  const auto plan = mft::mx4_plan(a.M, a.N, a.K, dgrad, (int)x2.size(1));
   Tensor ws;
   if (plan.dense) {
-    ws = torch::empty({N * K}, x.options());
+    ws = torch::empty({mft::mx4_dense_ws_elems(a.N, K, dgrad)}, x.options());
     mft::mx4_dense(a, bp(ws), dgrad, stream());
     return y;
   }

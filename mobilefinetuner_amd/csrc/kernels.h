@@ -415,10 +415,14 @@ struct Mx4Plan {
   int bm, tn, splits;  // rows and 64-column strips of a tile, workgroups that share a tile's reduction
   int dense;
 };
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits = 32, bool dense = true);
+// xcols: columns of x that may be read, zeros past its width
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, int xcols, int max_splits = 32, bool dense = true);
 long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad);
 void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t st);
-bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx);
+bool mx4_dense_supported(int M, int N, int K, bool dgrad, int xcols);
+long mx4_dense_ws_elems(int N, int K, bool dgrad);
+// rows of any address and stride, copied with zeros past their width (out 16-byte aligned, ldo % 8 == 0)
+void mx4_pad_rows(const bf16_t* in, long ldi, long rows, int width, bf16_t* out, int ldo, hipStream_t st);
 void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st);
 
 // ---------------------------------------------------------------- misc (misc.hip)

@@ -98,6 +98,26 @@ __global__ __launch_bounds__(256) void mx4_embed_kernel(const int64_t* __restric
   store8(out + m * K + c8 * 8, f);
 }
 
+// out[r, 0 : ldo] = in[r, 0 : width] and zeros, for rows of any 2-byte address and stride (ldo % 8 == 0, out aligned)
+__global__ __launch_bounds__(256) void mx4_pad_rows_kernel(const bf16_t* __restrict__ in, long ldi, long rows, int width,
+                                                           bf16_t* __restrict__ out, int ldo) {
+  const int l8 = ldo / 8;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * l8) return;
+  const long r = i / l8;
+  const int c = (int)(i - r * l8) * 8;
+  const bf16_t* p = in + r * ldi + c;
+  u16x8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (c + 8 <= width) {
+    __builtin_memcpy(&v, p, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < width) v[j] = p[j];
+  }
+  *reinterpret_cast<u16x8_t*>(out + r * ldo + c) = v;
+}
+
 // ------------------------------------------------------------------ y = x W^T + b, few rows
 // A wave owns TN * 16 output columns (rows n of W) and MT * 16 rows of x.  Per 128 columns of K a lane loads 16 B
 // of codes -- one scale group -- of row n = n0 + (l & 15), columns 32 (l >> 4) .. + 31, and turns it into the
@@ -198,12 +218,12 @@ __global__ __launch_bounds__(64 * (S > 4 ? S : 4)) void mx4_rows_kernel(Mx4Linea
       const int m = i * 16 + r16, nc = n0 + j * 16 + 4 * kq;
       if (m >= g.M || nc >= g.N) continue;
       bf16_t* y = g.y + (long)m * g.ldy + nc;
-      if (nc + 4 <= g.N && g.ldy % 4 == 0) {  // 8-byte rows and columns
+      if (nc + 4 <= g.N) {
         if (g.bias) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] += bf2f(g.bias[nc + r]);
         }
-        *reinterpret_cast<uint2*>(y) = uint2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+        store4_any(y, v);
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -304,12 +324,12 @@ __global__ __launch_bounds__(256) void mx4_stream_kernel(Mx4LinearArgs g) {
     if (nc >= g.N) continue;
     bf16_t* y = g.y + (long)r16 * g.ldy + nc;
     f32x4_t v = acc[j];
-    if (nc + 4 <= g.N && g.ldy % 4 == 0) {
+    if (nc + 4 <= g.N) {
       if (g.bias) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += bf2f(g.bias[nc + r]);
       }
-      *reinterpret_cast<uint2*>(y) = uint2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+      store4_any(y, v);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -351,6 +371,13 @@ void mx4_embed(const int64_t* ids, const uint8_t* codes, const uint8_t* scales, 
   check_grid(blocks, "mx4_embed");
   mx4_embed_kernel<<<(unsigned)blocks, 256, 0, st>>>(ids, reinterpret_cast<const uint32_t*>(codes), scales, N, K, wpe, out, M,
                                                      S, scale);
+}
+
+void mx4_pad_rows(const bf16_t* in, long ldi, long rows, int width, bf16_t* out, int ldo, hipStream_t st) {
+  const long n = rows * (ldo / 8), blocks = (n + 255) / 256;
+  if (n <= 0) return;
+  check_grid(blocks, "mx4_pad_rows");
+  mx4_pad_rows_kernel<<<(unsigned)blocks, 256, 0, st>>>(in, ldi, rows, width, out, ldo);
 }
 
 template <int MT, int TN, int S, int U>

@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
         const int m = m0 + i * 16 + r16, c = cw + j * 16 + 4 * kq;
         if (m >= g.M) continue;
         float* p = P + (long)m * cols + c;
-        if (c + 4 <= cols && cols % 4 == 0) *reinterpret_cast<f32x4_t*>(p) = acc[i][j];
+        if (c + 4 <= cols) __builtin_memcpy(p, &acc[i][j], 16);
         else
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -290,14 +290,20 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
       }
     return;
   }
-  const bool wide = TN > 1 && cols % 8 == 0 && g.ldy % 8 == 0;
-  if (wide) {
+  if constexpr (TN > 1) {
     const int cofs = (kq & 1) * 16 + (kq >> 1) * 8;
 #pragma unroll
     for (int j = 0; j + 1 < TN; j += 2) {
       const int c = cw + j * 16 + cofs;
       float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (!DG && g.bias && c < cols) load8(g.bias + c, bias);
+      const bool whole = c + 8 <= cols;
+      if (!DG && g.bias) {
+        if (whole) load8(g.bias + c, bias);
+        else
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (c + r < cols) bias[r] = bf2f(g.bias[c + r]);
+      }
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int m = m0 + i * 16 + r16;
@@ -308,7 +314,13 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
           o[r] = __uint_as_float(sw[0]) + bias[r];
           o[4 + r] = __uint_as_float(sw[1]) + bias[4 + r];
         }
-        if (m < g.M && c < cols) store8(g.y + (long)m * g.ldy + c, o);
+        if (m >= g.M) continue;
+        bf16_t* y = g.y + (long)m * g.ldy + c;
+        if (whole) store8_any(y, o);
+        else
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (c + r < cols) y[r] = f2bf(o[r]);
       }
     }
     return;
@@ -320,56 +332,76 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(Mx4LinearArgs g, int s
     for (int i = 0; i < MI; ++i) {
       const int m = m0 + i * 16 + r16;
       if (m >= g.M) continue;
+      f32x4_t v = acc[i][j];
+      if (!DG && g.bias) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (c + r < cols) g.y[(long)m * g.ldy + c + r] = f2bf(acc[i][j][r] + (!DG && g.bias ? bf2f(g.bias[c + r]) : 0.f));
+        for (int r = 0; r < 4; ++r)
+          if (c + r < cols) v[r] += bf2f(g.bias[c + r]);
+      }
+      bf16_t* y = g.y + (long)m * g.ldy + c;
+      if (c + 4 <= cols) store4_any(y, v);
+      else
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (c + r < cols) y[r] = f2bf(v[r]);
     }
   }
 }
 
-// y = the sum of the slabs in split order (+ bias), rounded once
-template <int V>
-__global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ ws, int splits, long M, int cols,
-                                                       const bf16_t* __restrict__ bias, bf16_t* __restrict__ y, long ldy) {
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * V, n = M * cols;
+// y = the sum of the slabs in split order (+ bias), rounded once; y and the slabs are contiguous, 4 values a lane
+__global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ ws, int splits, long n, int cols,
+                                                       const bf16_t* __restrict__ bias, bf16_t* __restrict__ y) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
-  float v[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = 0.f;
+  const int have = (int)min(4L, n - i);
+  f32x4_t v = zero4();
   for (int s = 0; s < splits; ++s) {
     const float* p = ws + s * n + i;
-    if constexpr (V == 4) {
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += a[e];
+    f32x4_t a = zero4();
+    if (have == 4) {
+      __builtin_memcpy(&a, p, 16);
     } else {
-      v[0] += p[0];
-    }
-  }
-  const long m = i / cols;
-  const int c = (int)(i - m * cols);
 #pragma unroll
-  for (int e = 0; e < V; ++e) y[m * ldy + c + e] = f2bf(v[e] + (bias ? bf2f(bias[c + e]) : 0.f));
+      for (int e = 0; e < 3; ++e)
+        if (e < have) a[e] = p[e];
+    }
+    v += a;
+  }
+  if (bias) {
+    const int c = (int)(i % cols);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < have) v[e] += bf2f(bias[(c + e) % cols]);
+  }
+  if (have == 4) {
+    store4_any(y + i, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < have) y[i + e] = f2bf(v[e]);
+  }
 }
 
-// W^T in bf16: out[k, n] for n < N (N % 64 == 0), 64 rows of W x 256 columns per workgroup.  The codes go through LDS
-// and come back transposed, as in the dx tiles; a lane writes 16 values of one row of W^T, four lanes 128 B.
+// W^T in bf16: out[k, n], n < Np = N rounded up to 64 (zeros past N), 64 rows of W x 256 columns per workgroup.  The codes
+// go through LDS and come back transposed, as in the dx tiles; a lane writes 16 values of one row of W^T, four lanes 128 B.
 __global__ __launch_bounds__(256) void mx4_dequant_t_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                            int N, int K, bf16_t* __restrict__ out) {
+                                                            int N, int Np, int K, bf16_t* __restrict__ out) {
   constexpr int CLD = 128 + 16;
   __shared__ __attribute__((aligned(16))) char img[64 * CLD];
   __shared__ __attribute__((aligned(16))) float sc[8 * 64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r16 = lane & 15, kq = lane >> 4;
   const int n0 = blockIdx.x * 64, c0 = blockIdx.y * 256, ng = K / 32;
-  const uint8_t* p = codes + (long)(n0 + (tid >> 2)) * (K / 2) + c0 / 2 + (tid & 3) * 32;
+  const bool in = n0 + (tid >> 2) < N;
+  const uint8_t* p = codes + (long)min(n0 + (tid >> 2), N - 1) * (K / 2) + c0 / 2 + (tid & 3) * 32;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
     if (c0 + (tid & 3) * 64 + e * 32 < K)
-      *reinterpret_cast<uint4*>(img + (tid >> 2) * CLD + (tid & 3) * 32 + e * 16) = *reinterpret_cast<const uint4*>(p + e * 16);
+      *reinterpret_cast<uint4*>(img + (tid >> 2) * CLD + (tid & 3) * 32 + e * 16) =
+          in ? *reinterpret_cast<const uint4*>(p + e * 16) : uint4{0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int id = e * 256 + tid, gi = c0 / 32 + (id & 7);
-    if (gi < ng) sc[(id & 7) * 64 + (id >> 3)] = mx4_scale(scales[(long)(n0 + (id >> 3)) * ng + gi]);
+    const int id = e * 256 + tid, gi = c0 / 32 + (id & 7), n = n0 + (id >> 3);
+    if (gi < ng) sc[(id & 7) * 64 + (id >> 3)] = n < N ? mx4_scale(scales[(long)n * ng + gi]) : 1.f;
   }
   __syncthreads();
 #pragma unroll
@@ -379,7 +411,7 @@ __global__ __launch_bounds__(256) void mx4_dequant_t_kernel(const uint8_t* __res
     const float* s = sc + ((w * 4 + j) >> 1) * 64 + kq * 16;
     const int k = c0 + (w * 4 + j) * 16 + r16;
     if (k >= K) continue;
-    bf16x8_t* o = reinterpret_cast<bf16x8_t*>(out + (long)k * N + n0 + kq * 16);
+    bf16x8_t* o = reinterpret_cast<bf16x8_t*>(out + (long)k * Np + n0 + kq * 16);
     o[0] = mx4_cvt8((uint32_t)raw[0], *reinterpret_cast<const f32x4_t*>(s), *reinterpret_cast<const f32x4_t*>(s + 4));
     o[1] = mx4_cvt8((uint32_t)raw[1], *reinterpret_cast<const f32x4_t*>(s + 8), *reinterpret_cast<const f32x4_t*>(s + 12));
   }
@@ -431,7 +463,7 @@ constexpr TileCost kCostDx[] = {{128, 4, 1.32f, 0.81f, 2.1f}, {128, 2, 0.83f, 0.
 
 }  // namespace
 
-Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits, bool dense) {
+Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, int xcols, int max_splits, bool dense) {
   if (K < 128) return Mx4Plan{64, 2, 1, 0};  // the narrow kernel
   const long cols = dgrad ? K : N, red = dgrad ? N : K;
   Mx4Plan best{};
@@ -454,7 +486,7 @@ Mx4Plan mx4_plan(int M, int N, int K, bool dgrad, long ldx, int max_splits, bool
     for (const TileCost& c : kCostY) consider(c);
   // through a bf16 copy: its writing and reading at 4.5 TB/s, then 256 x 256 tiles of gemm4 in K steps of 64 -- 1.15 us alone
   // on a CU, 1.5 us when every CU is busy -- and about 4 us per round of tiles
-  if (dense && mx4_dense_supported(M, N, K, dgrad, ldx)) {
+  if (dense && mx4_dense_supported(M, N, K, dgrad, xcols)) {
     const double tiles = (double)((M + 255L) / 256 * ((cols + 255) / 256)), rounds = std::ceil(tiles / 256), st = red / 64.0;
     const double t = 5 + (double)N * K * 2.53 / 4.5e6 + std::max(rounds * (st * 1.15 + 4), tiles / 256 * (st * 1.5 + 1));
     if (t < best_t) best = Mx4Plan{0, 0, 1, 1};
@@ -466,9 +498,12 @@ long mx4_plan_ws_floats(const Mx4Plan& p, int M, int N, int K, bool dgrad) {
   return p.splits > 1 ? (long)p.splits * M * (dgrad ? K : N) : 0;
 }
 
-bool mx4_dense_supported(int M, int N, int K, bool dgrad, long ldx) {
-  return ldx % 8 == 0 && (dgrad ? gemm4_supported(M, K, N, false, false) && K % 8 == 0 : gemm4_supported(M, N, K, false, false));
+bool mx4_dense_supported(int M, int N, int K, bool dgrad, int xcols) {
+  const int Np = (N + 63) / 64 * 64;
+  return dgrad ? xcols >= Np && gemm4_supported(M, K, Np, false, false) : gemm4_supported(M, N, K, false, false);
 }
+
+long mx4_dense_ws_elems(int N, int K, bool dgrad) { return (long)(dgrad ? (N + 63) / 64 * 64 : N) * K; }
 
 void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st) {
   GemmArgs f{};
@@ -477,8 +512,9 @@ void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st) {
   f.C = a.y; f.ldc = a.ldy;
   f.M = a.M; f.alpha = 1.f;
   if (dgrad) {
-    mx4_dequant_t_kernel<<<dim3(a.N / 64, (a.K + 255) / 256), 256, 0, st>>>(a.codes, a.scales, a.N, a.K, w);
-    f.ldb = a.N; f.N = a.K; f.K = a.N;
+    const int Np = (a.N + 63) / 64 * 64;
+    mx4_dequant_t_kernel<<<dim3(Np / 64, (a.K + 255) / 256), 256, 0, st>>>(a.codes, a.scales, a.N, Np, a.K, w);
+    f.ldb = Np; f.N = a.K; f.K = Np;
     gemm4x(f, GEMM_EPI_NONE, false, false, st);
   } else {
     mx4_dequantize(a.codes, a.scales, 0, a.N, a.K, w, a.K, a.N, a.K, st);
@@ -510,8 +546,7 @@ void mx4_tiles(const Mx4LinearArgs& a, const Mx4Plan& p, bool dgrad, hipStream_t
     const int cols = dgrad ? a.K : a.N;
     const long n = (long)a.M * cols;
     const bf16_t* bias = dgrad ? nullptr : a.bias;
-    if (cols % 4 == 0) mx4_join_kernel<4><<<(unsigned)((n / 4 + 255) / 256), 256, 0, st>>>(a.ws, p.splits, a.M, cols, bias, a.y, a.ldy);
-    else mx4_join_kernel<1><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a.ws, p.splits, a.M, cols, bias, a.y, a.ldy);
+    mx4_join_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(a.ws, p.splits, n, cols, bias, a.y);
   }
 }
 

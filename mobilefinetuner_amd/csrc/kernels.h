@@ -399,8 +399,8 @@ struct Mx4LinearArgs {
   const uint8_t* scales;
   const bf16_t* x;  // linear: x [M, K]; dgrad: dy [M, N] (N % 8 == 0, or its columns N .. up to 8 are zeros)
   long ldx;         // % 8 == 0, 16-B aligned rows
-  const bf16_t* bias;  // linear: [N] or null
-  bf16_t* y;        // linear: y [M, N]; dgrad: dx [M, K] (ldy % 4 == 0, 8-B aligned)
+  const bf16_t* bias;  // linear: [N], 16-B aligned, or null
+  bf16_t* y;        // linear: y [M, N]; dgrad: dx [M, K]; contiguous
   long ldy;
   int M, N, K;
   float* ws;  // mx4_plan_ws_floats
@@ -410,7 +410,7 @@ struct Mx4LinearArgs {
 int mx4_few_rows(int M, int N, int K);
 void mx4_rows(const Mx4LinearArgs& a, hipStream_t st);
 // y, or dx = dy W, by tiles that convert the weight in registers, or (dense) through a bf16 copy of W (of W^T for dx,
-// N * K elements) and gemm4 (mx4_gemm.hip).  The plan goes by the sizes alone.
+// mx4_dense_ws_elems) and gemm4 (mx4_gemm.hip).  The plan goes by the sizes alone.
 struct Mx4Plan {
   int bm, tn, splits;  // rows and 64-column strips of a tile, workgroups that share a tile's reduction
   int dense;

@@ -398,3 +398,21 @@ def test_codes_past_4_gib():
     out = Fx.mx4_embedding(ids, w4)
     assert torch.equal(out[0], v[-1].bfloat16()) and torch.equal(out[1], v[0].bfloat16()) and out[2].abs().max().item() == 0.0
     assert torch.equal(Fx.mx4_quantize(end.dequantize()).dequantize(), end.dequantize())
+
+
+@pytest.mark.parametrize("m,n,k", [(5000, 1603, 1600), (8236, 195, 1536), (700, 1001, 512), (20, 13001, 256), (3, 13003, 128), (50, 2047, 96)])
+def test_widths_that_are_no_multiple_of_8(m, n, k):
+    """Odd result rows, and the gradient of one that starts at an odd address in a larger tensor, as a copy gives it."""
+    Fx = _fx()
+    w4 = _weight(n, k, seed=m)
+    x = torch.randn(m, k, device="cuda", generator=_gen(n)).bfloat16().requires_grad_(True)
+    b = torch.randn(n, device="cuda", generator=_gen(k)).bfloat16()
+    big = torch.randn(m, n + 5, device="cuda", generator=_gen(k + 1)).bfloat16()
+    y = Fx.mx4_linear(x, w4, b)
+    dy = big[:, 3:3 + n]
+    (dx,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    (again,) = torch.autograd.grad(y, x, dy.contiguous())
+    v, xd, dd = ref.values(w4.codes, w4.scales).cuda(), x.detach().double(), dy.double()
+    _check(y.detach(), xd @ v.t() + b.double(), xd.abs() @ v.abs().t() + b.double().abs(), k)
+    _check(dx, dd @ v, dd.abs() @ v.abs(), n)
+    assert torch.equal(dx, again)

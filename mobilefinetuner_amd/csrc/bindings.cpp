@@ -332,8 +332,11 @@ std::pair<long, int> mx4_shape(const Tensor& codes, const Tensor& scales, const 
   return {N, (int)K};
 }
 const uint8_t* u8p(const Tensor& t) { return t.data_ptr<uint8_t>(); }
-bool rows16(const Tensor& t) {  // 2-D bf16 rows that 16-byte loads may walk, apart by less than 2^22 elements
-  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) < (1 << 22) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+// 2-D bf16 rows that 16-byte loads may walk, apart by less than 2^22 elements and by no less than their width: gemm4 bounds an
+// operand by rows x stride, so rows that repeat (stride 0, an expanded row) or overlap would be cut off there
+bool rows16(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && t.stride(0) < (1 << 22) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
 std::vector<Tensor> mx4_quantize(Tensor w) {

@@ -325,3 +325,19 @@ def test_backward_twice():
     (a,) = torch.autograd.grad(loss, x, retain_graph=True)
     (b,) = torch.autograd.grad(loss, x)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m", [1, 5, 300])
+@pytest.mark.parametrize("table", ["bf16", "mx4"])
+@pytest.mark.parametrize("stride", [0, 8])
+def test_rows_that_repeat_or_overlap(m, table, stride):
+    """h whose rows are all one row or start 8 elements apart (a one-row h with a row stride below its width, too), and a
+    bf16 table whose rows overlap."""
+    k, v = 128, 900
+    g = torch.Generator(device="cuda").manual_seed(m + stride)
+    _, w, wd, labels = _case(m, k, v, table, seed=m, ignore=0.0)
+    h = torch.randn((m - 1) * stride + k, device="cuda", generator=g).bfloat16().as_strided((m, k), (stride, 1))
+    _check(h, w, wd, labels, v, 512)
+    if table == "bf16" and stride:
+        w = (torch.randn((v - 1) * stride + k, device="cuda", generator=g) * k ** -0.5).bfloat16().as_strided((v, k), (stride, 1))
+        _check(h, w, w.double(), labels, v, 512)

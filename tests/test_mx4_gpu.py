@@ -416,3 +416,29 @@ def test_widths_that_are_no_multiple_of_8(m, n, k):
     _check(y.detach(), xd @ v.t() + b.double(), xd.abs() @ v.abs().t() + b.double().abs(), k)
     _check(dx, dd @ v, dd.abs() @ v.abs(), n)
     assert torch.equal(dx, again)
+
+
+# ---------------------------------------------------------------- rows that repeat or overlap, at sizes of the bf16 copy
+@pytest.mark.parametrize("m,n,k", [(9000, 6400, 1600), (600, 136, 192), (7, 96, 64)])
+@pytest.mark.parametrize("stride", [0, 8])
+def test_rows_that_repeat_or_overlap(m, n, k, stride):
+    """x and dy whose rows are all one row (an expanded one) or start 8 elements apart, and the gradient that a sum over the
+    rows hands back, strides (0, 1)."""
+    Fx = _fx()
+    w4 = _weight(n, k, seed=m)
+    v = ref.values(w4.codes, w4.scales).cuda()
+
+    def rows(width, seed):
+        flat = torch.randn((m - 1) * stride + width, device="cuda", generator=_gen(seed)).bfloat16()
+        return flat.as_strided((m, width), (stride, 1))
+    x = rows(k, n).detach().requires_grad_(True)
+    xd = x.detach().double()
+    y = Fx.mx4_linear(x, w4)
+    _check(y.detach(), xd @ v.t(), xd.abs() @ v.abs().t(), k)
+    dy = rows(n, k)
+    (dx,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    _check(dx, dy.double() @ v, dy.double().abs() @ v.abs(), n)
+    g = torch.randn(n, device="cuda", generator=_gen(11)).bfloat16()
+    (dx,) = torch.autograd.grad(y.sum(0), x, g)
+    want = (g.double() @ v).expand(m, k)
+    _check(dx, want, (g.double().abs() @ v.abs()).expand(m, k), n)

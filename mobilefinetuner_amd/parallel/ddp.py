@@ -46,6 +46,21 @@ def rank():
     return dist.get_rank() if is_dist() else 0
 
 
+def drain_collectives(*groups):
+    """Before a graph capture: wait until every collective issued so far on the default group and on ``groups`` has run and
+    RCCL's watchdog thread is done with it.  The watchdog looks at its list of eager collectives every 100 ms and queries the
+    event recorded behind each on RCCL's stream.  That stream takes part in the capture of a step that records collectives,
+    and HIP refuses the query of an event on a capturing stream (hipErrorCapturedEvent), in every capture mode: the watchdog
+    throws, which ends the process, while the capture itself goes on where all its collectives are joined already.  (Recorded
+    collectives are not on the watchdog's list.)"""
+    if not is_dist():
+        return
+    torch.cuda.synchronize()
+    for pg in {g if g is not None else dist.distributed_c10d._get_default_group() for g in (None, *groups)}:
+        if _supports_avg(pg):
+            pg._wait_for_pending_works()
+
+
 def _supports_avg(group=None):
     try:
         return dist.get_backend(group) == "nccl"
@@ -89,13 +104,9 @@ class DataParallel:
         self.overlap = overlap and self.active
         # collectives recorded into the step's hipGraph from the backward's grad-ready hooks: the
         # default on RCCL (MFT_GRAPH_COMM=0 reduces the buckets eagerly after the replay instead).
-        # Round 2 kept it opt-in after captures aborted intermittently at capture end on a 1-rank
-        # group; round 3 re-ran the recorded-collective tests (DDP, bf16, ZeRO-2:
-        # tests/test_dp_graph_gpu.py::test_reducer_with_graph_step_matches_no_dp, part of the 184 GPU
-        # tests passing in profiles/r3_final_gpu_tests.log) without an abort and found RCCL's AVG
-        # inexact at some lengths (profiles/r3_rccl_avg_tail.txt), which is
-        # no longer used (sum + divide).  The capture runs in thread_local mode so RCCL's watchdog
-        # thread polling earlier events cannot invalidate it (train/engine.py).
+        # Captures on a 1-rank group have aborted now and then, in RCCL's watchdog thread: the eager steps'
+        # collectives were still on its list when the capture began.  drain_collectives() waits for them, and
+        # the capture runs in thread_local mode (train/engine.py).
         self.capturable = self.nccl and os.environ.get("MFT_GRAPH_COMM", "1") == "1"
         self.shard = shard
         cap = int(bucket_mb * (1 << 20) / 4)

@@ -15,7 +15,7 @@ import torch
 
 from ..optim.adamw import FusedAdamW
 from ..utils.trace import trace_range
-from ..parallel.ddp import DataParallel
+from ..parallel.ddp import DataParallel, drain_collectives
 from ..utils.params import FlatParams
 
 
@@ -81,6 +81,7 @@ class TrainStep:
     # ----------------------------------------------------------------- graph capture
     def _capture(self, batches):
         dev = self.flat.grad.device
+        drain_collectives(getattr(self.dp, "group", None))
         self._static = [(ids.clone(), lab.clone()) for ids, lab in batches]
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -88,9 +89,8 @@ class TrainStep:
         with torch.cuda.stream(side):
             if self.dp is not None:
                 self.dp.begin_step()
-            # thread_local: RCCL's watchdog thread keeps polling the events of earlier collectives
-            # while this thread captures; under the default "global" mode those hipEventQuery
-            # calls fail (hipErrorStreamCaptureUnsupported) and abort the process group
+            # thread_local: what other threads of the process call (RCCL's watchdog, data loading)
+            # must not fail or end this capture; in the default "global" mode it does
             with torch.cuda.graph(self.graph, stream=side, capture_error_mode="thread_local"):
                 self._fwd_bwd(self._static)
                 if self.graph_comm:

@@ -6,8 +6,11 @@
 //   2. ce_piece_finalize: the running row maximum M' and sum S' over the pieces so far, the factor
 //      exp(M - M') that rescales what earlier pieces added, the dgrad's per-tile factors;
 //   3. the gradient product A' = A exp(M - M') + sum_v exp(l_v - M') W_v in fp32.
-// At the end, with lse = M + log S and p the label's probability,
-//   loss = lse - l_label,   dh = w (A / S - (1 - p) W_label),   w = 1 / valid rows,
+// E is bf16 because the matrix cores multiply bf16: each softmax number is off by at most half a step (2^-8 of it).
+// Maxima are held in units of log 2, m log2(e) rounded to fp32 as the epilogue rounds it: E and the sums are relative to that
+// rounded number (at a logit of 1000 it is 6e-5 beside the maximum), so every factor between tiles uses it too.
+// At the end, with p the label's probability and d = l_label log2(e) - M (one fma: exact where the label is the maximum),
+//   loss = log S - d log 2,   dh = w (A / S - (1 - p) W_label),   w = 1 / valid rows,
 // the label's own column being left out of A (its E is set to 0): a row that is sure of its label has p near 1,
 // and (p - 1) W_label from a p rounded to bf16 would drown the small gradient that is left.
 // A 4-bit table is turned into bf16 one piece at a time, in a workspace of P rows.
@@ -22,6 +25,15 @@
 namespace mft {
 
 namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// a logit in units of log 2, rounded by itself (the empty asm keeps a later subtraction from taking the product into an fma)
+__device__ __forceinline__ float log2_units(float l) {
+  float p = l * kLog2e;
+  asm("" : "+v"(p));
+  return p;
+}
 
 // a row's position inside its 256-row tile in the order the CE dgrad reads its row factors (gemm8.hip)
 __device__ __forceinline__ long ratio_pos(int R) {
@@ -59,9 +71,9 @@ __device__ __forceinline__ float count_valid(const float* counts, int M) {
 }
 
 // RB rows per block.  Pass 1 (a wave per row, lanes over the piece's tiles): the piece's maximum and sum join the
-// running ones.  Pass 2: ratio[t][row] = exp(m'_{t-1} - m'_t) with m'_t = max(m_t, M' - 60) -- a tile 60 below the
-// maximum adds less than e^-60, and the clamp keeps every factor and partial sum finite in fp32 -- staged through
-// LDS so that reads run over tiles and writes over rows.
+// running ones.  Pass 2: ratio[t][row] = 2^(m'_{t-1} - m'_t) with m'_t = max(m_t, M' - 86): the clamp keeps every factor and
+// partial sum finite in fp32, and a tile further below the maximum, weighted 2^-86, adds at most 256 x 2^-86 of its share
+// -- staged through LDS so that reads run over tiles and writes over rows.
 template <int RB>
 __global__ __launch_bounds__(256) void ce_piece_finalize_kernel(const float2* __restrict__ stats, int M, int T, long mpad,
                                                                 const int64_t* __restrict__ labels, int next0, int next_w,
@@ -78,20 +90,20 @@ __global__ __launch_bounds__(256) void ce_piece_finalize_kernel(const float2* __
     if (R >= M) break;
     const float2* st = stats + (long)R * T;
     float m = -INFINITY;
-    for (int t = lane; t < T; t += 64) m = fmaxf(m, st[t].x);
+    for (int t = lane; t < T; t += 64) m = fmaxf(m, log2_units(st[t].x));
     const float m0 = run_m[R];
     m = fmaxf(wave_max(m), m0);
     float s = 0.f;
     for (int t = lane; t < T; t += 64) {
       const float2 v = st[t];
-      s += v.y == 0.f ? 0.f : v.y * __expf(v.x - m);
+      s += v.y == 0.f ? 0.f : v.y * fast_exp2(log2_units(v.x) - m);
     }
     s = wave_sum(s);
-    const float back = m0 == -INFINITY ? 0.f : __expf(m0 - m);
+    const float back = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m);
     if (fin)
       for (int sp = lane; sp < nsplit; sp += 64) {
         const int te = min((sp + 1) * tps, T) - 1;
-        fin[(long)sp * M + R] = __expf(fmaxf(st[te].x, m - 60.f) - m);
+        fin[(long)sp * M + R] = fast_exp2(fmaxf(log2_units(st[te].x), m - 86.f) - m);
       }
     if (lane == 0) {
       s_mx[rr] = m;
@@ -113,10 +125,10 @@ __global__ __launch_bounds__(256) void ce_piece_finalize_kernel(const float2* __
   for (int c0 = 0; c0 < T - 1; c0 += 63) {
     const int cn = min(64, T - c0);
     for (int rr = w; rr < nrow; rr += 4)
-      if (lane < cn) s_m[rr][lane] = fmaxf(stats[(long)(r0 + rr) * T + c0 + lane].x, s_mx[rr] - 60.f);
+      if (lane < cn) s_m[rr][lane] = fmaxf(log2_units(stats[(long)(r0 + rr) * T + c0 + lane].x), s_mx[rr] - 86.f);
     __syncthreads();
     if (rr2 < nrow)
-      for (int j = 1 + jg; j < cn; j += 256 / RB) ratio[(long)(c0 + j) * mpad + dst] = __expf(s_m[rr2][j - 1] - s_m[rr2][j]);
+      for (int j = 1 + jg; j < cn; j += 256 / RB) ratio[(long)(c0 + j) * mpad + dst] = fast_exp2(s_m[rr2][j - 1] - s_m[rr2][j]);
     __syncthreads();
   }
 }
@@ -151,7 +163,8 @@ __global__ __launch_bounds__(256) void ce_pieces_rows_kernel(const float* __rest
   if (R >= M) return;
   const int64_t lab = labels[R];
   const bool valid = lab >= 0 && lab < V;
-  const float s = run_s[R], lse = run_m[R] + __logf(s), nll = lse - lbl[R];
+  // log S near 1 keeps the bits that a loss formed from numbers of the logits' size would drop (4e-6 at 64, 6e-5 at 1024)
+  const float s = run_s[R], d = fmaf(lbl[R], kLog2e, -run_m[R]), nll = logf(s) - d * kLn2;
   if (lane == 0 && ws == 0) loss_rows[R] = valid ? nll : 0.f;
   if (!dh) return;
   const float wt = 1.f / fmaxf(count_valid(counts, M), 1.f), fa = wt / s, fl = wt * -expm1f(-nll);  // 1 - p = 1 - exp(l - lse)
@@ -215,7 +228,7 @@ __global__ __launch_bounds__(1024) void ce_pieces_loss_kernel(const float* __res
 }
 
 // ---- few rows on a 4-bit table: fp32 logits of a piece from the 4-bit tiles, these two kernels, the 4-bit gradient tiles.
-// (row, 2,048 columns) per workgroup: maximum and sum of exp(l - maximum)
+// (row, 2,048 columns) per workgroup: maximum and sum of exp(l - maximum), relative to the maximum as log2_units rounds it
 constexpr int kChunk = 2048;
 __global__ __launch_bounds__(256) void ce_few_stats_kernel(const float* __restrict__ logits, int W,
                                                            float2* __restrict__ stats) {
@@ -230,11 +243,12 @@ __global__ __launch_bounds__(256) void ce_few_stats_kernel(const float* __restri
     m = fmaxf(m, v[i]);
   }
   m = block_max(m, red);
+  const float mb = log2_units(m);
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kChunk / 256; ++i) s += v[i] == -INFINITY ? 0.f : __expf(v[i] - m);
+  for (int i = 0; i < kChunk / 256; ++i) s += v[i] == -INFINITY ? 0.f : fast_exp2(fmaf(v[i], kLog2e, -mb));
   s = block_sum(s, red);
-  if (threadIdx.x == 0) stats[(long)blockIdx.y * gridDim.x + blockIdx.x] = float2{m, s};
+  if (threadIdx.x == 0) stats[(long)blockIdx.y * gridDim.x + blockIdx.x] = float2{mb, s};
 }
 
 // The row's running maximum and sum over the pieces so far (old state -> new state, by the row's first workgroup), the
@@ -256,10 +270,10 @@ __global__ __launch_bounds__(256) void ce_few_exp_kernel(const float* __restrict
   const float* l = logits + (long)R * W;
   if (blockIdx.x == 0) {
     float s = 0.f;
-    for (int i = threadIdx.x; i < C; i += 256) s += st[i].y == 0.f ? 0.f : st[i].y * __expf(st[i].x - m);
+    for (int i = threadIdx.x; i < C; i += 256) s += st[i].y == 0.f ? 0.f : st[i].y * fast_exp2(st[i].x - m);
     s = block_sum(s, red);
     if (threadIdx.x == 0) {
-      const float back = m0 == -INFINITY ? 0.f : __expf(m0 - m);
+      const float back = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m);
       run_m[R] = m;
       run_s[R] = old_s[R] * back + s;
       accscale[R] = back;
@@ -272,7 +286,8 @@ __global__ __launch_bounds__(256) void ce_few_exp_kernel(const float* __restrict
   for (int i = 0; i < kChunk / 512; ++i) {  // pairs of columns
     const int c = c0 + (i * 256 + threadIdx.x) * 2;
     if (c >= lde) continue;
-    const float a = c < W && c != rel ? __expf(l[c] - m) : 0.f, b = c + 1 < W && c + 1 != rel ? __expf(l[c + 1] - m) : 0.f;
+    const float a = c < W && c != rel ? fast_exp2(fmaf(l[c], kLog2e, -m)) : 0.f,
+                b = c + 1 < W && c + 1 != rel ? fast_exp2(fmaf(l[c + 1], kLog2e, -m)) : 0.f;
     *reinterpret_cast<uint32_t*>(E + R * lde + c) = pack_bf2(a, b);
   }
 }

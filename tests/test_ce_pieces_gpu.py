@@ -341,3 +341,39 @@ def test_rows_that_repeat_or_overlap(m, table, stride):
     if table == "bf16" and stride:
         w = (torch.randn((v - 1) * stride + k, device="cuda", generator=g) * k ** -0.5).bfloat16().as_strided((v, k), (stride, 1))
         _check(h, w, w.double(), labels, v, 512)
+
+
+@pytest.mark.parametrize("m,piece", [(6, None), (300, None), (300, 256)])
+@pytest.mark.parametrize("table", ["bf16", "mx4"])
+def test_sure_rows_of_large_logits(m, piece, table):
+    """Rows whose label lies at a logit of 1040, 10 to 22 above every other: the gradient that is left, about 5e-4, keeps its
+    precision although an fp32 number of that size has steps of 1.2e-4.  Every number is a small multiple of a power of two,
+    so the logits are exact, and what remains of the room is
+    - off the label: p rounded to bf16 (2^-8), the exponential of a difference up to 32 (2^-17), the fp32 sum (v 2^-23);
+    - at the label 1 - p = 1 - 1 / S: S = 1 + the others' sum, with fewer than 64 additions to a partial sum of about 1 (2^-18);
+    - one rounding of the result (2^-8)."""
+    k, v = 128, 1500
+    g = torch.Generator(device="cuda").manual_seed(m)
+    sign = torch.randint(0, 2, (v, k), device="cuda", generator=g) * 2.0 - 1.0
+    w = 0.5 * sign
+    w[:, 0] = 4.0
+    labels = torch.randint(0, v, (m,), device="cuda", generator=g)
+    h = (0.25 * sign[labels]).bfloat16()
+    h[:, 0] = 256.0
+    wd = w.double()
+    w = _fx().mx4_quantize(w) if table == "mx4" else w.bfloat16()
+    if table == "mx4":
+        assert torch.equal(w.dequantize().double(), wd)
+    loss, dh = _run(h, w, labels, v, piece)
+    logits = h.double() @ wd.t()
+    top = logits.gather(1, labels[:, None])
+    off = torch.exp(logits - top).scatter(1, labels[:, None], 0.0)
+    tail = off.sum(1, keepdim=True)
+    assert (tail < 1e-2).all() and (top > 1030).all()
+    p, rest = off / (1 + tail), tail / (1 + tail)
+    want = (p @ wd - rest * wd[labels]) / m
+    room = ((p @ wd.abs()) * (2.0 ** -8 + 2.0 ** -17 + v * 2.0 ** -23) + wd[labels].abs() * (2.0 ** -18 + rest * 2.0 ** -16)) / m
+    over = (dh.double() - want).abs() - (room + want.abs() * 2.0 ** -8 + 2.0 ** -133)
+    assert over.max().item() <= 0, over.max().item()
+    nll = torch.log1p(tail).mean().item()
+    assert abs(loss.item() - nll) <= 2.0 ** -18 + 2.0 ** -16 * nll, (loss.item(), nll)

@@ -507,7 +507,7 @@ std::vector<Tensor> lm_head_ce_pieces(Tensor h, c10::optional<Tensor> W, c10::op
   a.h = bp(h); a.ldh = h.stride(0);
   a.labels = labels.data_ptr<int64_t>();
   a.M = (int)M; a.K = (int)K; a.Kp = Kp; a.V = (int)V;
-  a.piece = piece ? (int)piece : mft::lm_head_ce_pieces_width(M, (int)V);
+  a.piece = (int)piece;
   a.loss = fp(loss); a.loss_rows = fp(rows); a.n_valid = n_valid.data_ptr<int64_t>();
   a.dh = grad ? bp(dh) : nullptr;
   auto ws = torch::empty({mft::lm_head_ce_pieces_ws_bytes(a)}, h.options().dtype(torch::kUInt8));
@@ -963,7 +963,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("mx4_dgrad", &mx4_dgrad);
   m.def("lm_head_ce_pieces", &lm_head_ce_pieces);
   m.def("lm_head_ce_pieces_grad", &lm_head_ce_pieces_grad, "the loss as an autograd node, gradient to h");
-  m.def("lm_head_ce_pieces_width", &mft::lm_head_ce_pieces_width, "default columns of a vocabulary piece for M rows");
+  m.def("lm_head_ce_pieces_width", &mft::lm_head_ce_pieces_width, py::arg("M"), py::arg("V"), py::arg("piece") = 0,
+        "columns of a vocabulary piece for M rows, the default or at most the ones asked for");
   m.def("sumsq", &sumsq);
   m.def("nonfinite_check", &nonfinite_check);
   m.def("adamw_step", &adamw_step, py::arg("p"), py::arg("g"), py::arg("m"), py::arg("v"), py::arg("lr"),

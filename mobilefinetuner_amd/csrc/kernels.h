@@ -252,7 +252,7 @@ struct CePiecesArgs {
   const uint8_t *codes, *scales;  // the 4-bit table [V, K]
   const int64_t* labels;       // [M]; outside [0, V): an ignored row
   int M, K, Kp, V;
-  int piece;                   // columns of a full piece (% 256 == 0)
+  int piece;                   // columns of a full piece wanted (% 256 == 0), 0: 2 GiB of E
   float* loss;                 // [1] mean over the valid rows (0 without any)
   float* loss_rows;            // [M], 0 for ignored rows
   int64_t* n_valid;            // [1]
@@ -260,7 +260,7 @@ struct CePiecesArgs {
   void* ws;                    // lm_head_ce_pieces_ws_bytes
 };
 long lm_head_ce_pieces_ws_bytes(const CePiecesArgs& a);
-int lm_head_ce_pieces_width(long M, int V);  // the default piece
+int lm_head_ce_pieces_width(long M, int V, int piece);  // columns of a full piece
 void lm_head_ce_pieces(const CePiecesArgs& a, hipStream_t st);
 // log-softmax gather: out[m, c] = logits[m, idx[c]] - lse(logits[m])  (MMLU scoring)
 void logsoftmax_gather(const bf16_t* logits, const int64_t* idx, float* out, long M, int V, long ld, int nidx,

@@ -360,7 +360,7 @@ Mx4Plan few_plan(const CePiecesArgs& a, int w) { return mx4_plan(a.M, w, a.K, tr
 
 Plan make_plan(const CePiecesArgs& a) {
   Plan p{};
-  p.width = std::min(a.piece, (a.V + 255) / 256 * 256);
+  p.width = lm_head_ce_pieces_width(a.M, a.V, a.piece);
   p.few = !a.W && a.M <= kFewRows && a.K >= 128;
   p.n = (a.V + p.width - 1) / p.width;
   p.last = a.V - (p.n - 1) * p.width;
@@ -427,11 +427,14 @@ Layout make_layout(const CePiecesArgs& a, const Plan& p) {
 
 }  // namespace
 
-int lm_head_ce_pieces_width(long M, int V) {
+int lm_head_ce_pieces_width(long M, int V, int piece) {
   // E [M, piece] bf16 of 2 GiB, at least 4,096 columns.  16384 x 262144 x 640 in ms by columns of a piece: 4,096 17.4,
   // 16,384 (512 MiB) 12.6, 65,536 (2 GiB) 11.5, the whole vocabulary (8 GiB) 11.5.
-  const long w = (2L << 30) / (2 * std::max(M, 1L)) / 256 * 256;
-  return (int)std::min(std::max(w, 4096L), (long)(V + 255) / 256 * 256);
+  M = std::max(M, 1L);
+  long w = piece ? piece : std::max((2L << 30) / (2 * M) / 256 * 256, 4096L);
+  // What the products address in 32 bits: 256 rows of E (2^21 columns: 1 GiB) and the statistics of all rows (8 B a tile).
+  w = std::min({w, 1L << 21, 0x7fffffffL / (8 * M) * 256});
+  return (int)std::min(w, (long)(V + 255) / 256 * 256);
 }
 
 long lm_head_ce_pieces_ws_bytes(const CePiecesArgs& a) {

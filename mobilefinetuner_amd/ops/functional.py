@@ -1158,11 +1158,12 @@ def lm_head_cross_entropy(h, w, labels, vocab_size, chunk=None, w_grad_scale=1.0
 def lm_head_cross_entropy_pieces(h, w, labels, vocab_size, piece=None):
     """Mean token NLL of logits = h W^T over the rows whose label lies in [0, vocab_size) (others, -100 among
     them, are ignored; none at all gives 0), swept in pieces of ``piece`` vocabulary columns (a multiple of
-    256; None: 2 GiB of bf16, by the row count): beside h, dh and fp32 partial sums of dh the memory is one
-    [rows, piece] bf16 buffer (up to 192 rows of a 4-bit table an fp32 one as well, else one bf16 piece of that
-    table), whatever the vocabulary -- lm_head_cross_entropy keeps one of the whole vocabulary's width.  W is
-    frozen: bf16 [>= vocab_size, C] (C a multiple of 8; rows past the vocabulary are not used) or
-    an MX4Weight; the gradient goes to h.  A trainable W is lm_head_cross_entropy's."""
+    256, narrower where rows x piece is too much for one sweep; None: 2 GiB of bf16, by the row count): beside
+    h, dh and fp32 partial sums of dh the memory is one [rows, piece] bf16 buffer (up to 192 rows of a 4-bit
+    table an fp32 one as well, else one bf16 piece of that table), whatever the vocabulary --
+    lm_head_cross_entropy keeps one of the whole vocabulary's width.  W is frozen: bf16 [>= vocab_size, C]
+    (C a multiple of 8; rows past the vocabulary are not used) or an MX4Weight; the gradient goes to h.  A
+    trainable W is lm_head_cross_entropy's."""
     if _needs(w):
         raise RuntimeError("lm_head_cross_entropy_pieces: W is frozen here; lm_head_cross_entropy trains it")
     mx = isinstance(w, MX4Weight)

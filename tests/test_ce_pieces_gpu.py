@@ -377,3 +377,14 @@ def test_sure_rows_of_large_logits(m, piece, table):
     assert over.max().item() <= 0, over.max().item()
     nll = torch.log1p(tail).mean().item()
     assert abs(loss.item() - nll) <= 2.0 ** -18 + 2.0 ** -16 * nll, (loss.item(), nll)
+
+
+def test_statistics_past_2_gib():
+    """300,000 rows x 262,144 columns in one piece, the loss alone: 2.4 GB of tile statistics if the piece stays whole.
+    The loss of the last rows, the others being ignored, against the formula."""
+    m, k, v, last = 300000, 128, 262144, 40
+    h, w, wd, labels = _case(m, k, v, "bf16", seed=14, ignore=0.0)
+    labels[:-last] = -100
+    loss = _fx().lm_head_cross_entropy_pieces(h, w, labels, v, v)
+    want, _, _, room = _exact(h[-last:], wd, labels[-last:])
+    assert abs(loss.item() - want.item()) <= room, (loss.item(), want.item(), room)

@@ -331,6 +331,13 @@ std::pair<long, int> mx4_shape(const Tensor& codes, const Tensor& scales, const 
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, what, ": codes must start at a 16-byte boundary");
   return {N, (int)K};
 }
+// these operators have no forward-mode derivative: a dual tensor (torch.autograd.forward_ad) is refused, its tangent would be lost
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, ": no forward-mode derivative");
+}
+void no_tangent(const c10::optional<Tensor>& t, const char* what) {
+  if (t.has_value()) no_tangent(*t, what);
+}
 const uint8_t* u8p(const Tensor& t) { return t.data_ptr<uint8_t>(); }
 // 2-D bf16 rows that 16-byte loads may walk, apart by less than 2^22 elements and by no less than their width: gemm4 bounds an
 // operand by rows x stride, so rows that repeat (stride 0, an expanded row) or overlap would be cut off there
@@ -368,6 +375,7 @@ Tensor mx4_embed(Tensor ids, Tensor codes, Tensor scales, c10::optional<Tensor> 
   TORCH_CHECK(ids.is_cuda() && ids.device() == codes.device() && ids.scalar_type() == torch::kInt64 && ids.dim() == 2,
               "mx4_embedding: ids [B, S] must be int64 on the table's GPU");
   TORCH_CHECK(N > 0, "mx4_embedding: the table has no rows");
+  no_tangent(wpe, "mx4_embedding");
   const long S = ids.size(1), M = ids.numel();
   if (wpe.has_value()) {
     TORCH_CHECK(wpe->is_cuda() && wpe->device() == codes.device() && wpe->scalar_type() == torch::kBFloat16 && wpe->dim() == 2 &&
@@ -400,6 +408,8 @@ Tensor mx4_product(const Tensor& x, const Tensor& codes, const Tensor& scales, c
   const auto [N, K] = mx4_shape(codes, scales, what);
   TORCH_CHECK(x.is_cuda() && x.device() == codes.device(), what, ": the activation must be on the weight's GPU");
   TORCH_CHECK(x.scalar_type() == torch::kBFloat16, what, ": the activation must be bf16");
+  no_tangent(x, what);
+  no_tangent(bias, what);
   const long in = dgrad ? N : K, out = dgrad ? K : N;
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) == in, what, ": expected [.., ", in, "], got ", x.sizes());
   if (bias.has_value() && bias->defined())
@@ -468,6 +478,8 @@ std::vector<Tensor> lm_head_ce_pieces(Tensor h, c10::optional<Tensor> W, c10::op
   const char* what = "lm_head_cross_entropy_pieces";
   CHECK_CUDA(h); CHECK_BF16(h);
   TORCH_CHECK(h.dim() == 2, what, ": h must be [M, C]");
+  no_tangent(h, what);
+  no_tangent(W, what);
   const long M = h.size(0), K = h.size(1);
   TORCH_CHECK(labels.is_cuda() && labels.device() == h.device() && labels.scalar_type() == torch::kInt64 && labels.numel() == M,
               what, ": labels must be int64 [M] on h's GPU");

@@ -442,3 +442,25 @@ def test_rows_that_repeat_or_overlap(m, n, k, stride):
     (dx,) = torch.autograd.grad(y.sum(0), x, g)
     want = (g.double() @ v).expand(m, k)
     _check(dx, want, (g.double().abs() @ v.abs()).expand(m, k), n)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad):
+    """A dual tensor's tangent is not dropped without a word, whether or not a gradient is tracked as well."""
+    import torch.autograd.forward_ad as fw
+    Fx = _fx()
+    w4 = _weight(64, 64)
+    ids = torch.zeros(1, 2, device="cuda", dtype=torch.long)
+    labels = torch.zeros(2, device="cuda", dtype=torch.long)
+    plain = torch.ones(2, 64, device="cuda", dtype=torch.bfloat16)
+    table = torch.ones(64, 64, device="cuda", dtype=torch.bfloat16)
+    with fw.dual_level():
+        x = fw.make_dual(plain.clone().requires_grad_(grad), torch.ones_like(plain))
+        b = fw.make_dual(torch.ones_like(plain[0]), torch.ones_like(plain[0]))
+        t = fw.make_dual(table.clone(), torch.ones_like(table))
+        for call in (lambda: Fx.mx4_linear(x, w4), lambda: Fx.mx4_linear(plain, w4, b), lambda: Fx.linear(x, w4),
+                     lambda: Fx.mx4_embedding(ids, w4, t), lambda: Fx.lm_head_cross_entropy_pieces(x, w4, labels, 64),
+                     lambda: Fx.lm_head_cross_entropy_pieces(x, table, labels, 64), lambda: Fx.lm_head_token_nll(x, w4, labels, 64),
+                     lambda: Fx.lm_head_cross_entropy_pieces(plain, t, labels, 64)):
+            with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                call()

@@ -3,7 +3,9 @@
 ``MX4Weight`` holds a matrix W [N, K] as e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two
 per byte with the even column in the low half, and one power-of-two scale per 32 columns of a row
 (2 ** (byte - 127); byte 255 reads as NaN): 4.25 bits a weight.  Sign, 1-bit mantissa and a power-of-two
-scale make every weight exact in bf16, so products with it round nothing but their result.
+scale make every weight exact in bf16, so products with it round nothing but their result.  ``mx4_quantize``
+writes bytes 2 to 252; in weights made elsewhere bytes 0 and 1 give denormal bf16 numbers, exact as well, and
+under bytes 253 and 254 a number past bf16's largest one reads as an infinity.
 
 It stands where a frozen weight tensor stands: ``Linear.weight``, a model's vocabulary table, and the
 ``w`` of ``ops.functional``'s linear, LoRA, embedding and LM-head loss ops.

@@ -464,3 +464,38 @@ def test_forward_mode_derivatives_are_refused(grad):
                      lambda: Fx.lm_head_cross_entropy_pieces(plain, t, labels, 64)):
             with pytest.raises(RuntimeError, match="forward-mode|jvp"):
                 call()
+
+
+# ---------------------------------------------------------------- scale bytes that the quantiser does not write
+def test_every_scale_byte_and_code():
+    """Bytes 0 and 1 (bf16 denormals), 253 and 254 (what is past bf16's largest number is an infinity), 255 (NaN), in weights
+    from elsewhere: each of the 16 codes under each of the 256 bytes."""
+    Fx = _fx()
+    c = torch.arange(16, dtype=torch.uint8)
+    codes = (c | ((c + 1) % 16) << 4).repeat(256, 1).cuda()
+    w4 = Fx.MX4Weight(codes, torch.arange(256, dtype=torch.uint8).view(256, 1).cuda())
+    want = ref.values(w4.codes, w4.scales).bfloat16()
+    ids = torch.arange(256, device="cuda").view(1, 256)
+    for got in (w4.dequantize(), Fx.mx4_embedding(ids, w4)):
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+        assert torch.equal(got.cpu()[:255], want[:255])
+
+
+@pytest.mark.parametrize("m,n", [(1, 64), (40, 64), (4, 13000), (300, 512), (9000, 6400)])
+@pytest.mark.parametrize("byte", [0, 1, 2])
+def test_smallest_scales_in_products(m, n, byte):
+    """Denormal bf16 weights reach the products of every route: one times 2^100, exact."""
+    from mobilefinetuner_amd._ext import native
+    Fx = _fx()
+    k = 128
+    codes = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda")
+    codes[:, 0] = 0x21  # 0.5 and 1
+    w4 = Fx.MX4Weight(codes, torch.full((n, k // 32), byte, dtype=torch.uint8, device="cuda"))
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    x[:, :2] = 2.0 ** 100
+    dy = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+    dy[:, 0] = 2.0 ** 100
+    scale = 2.0 ** (byte - 27)
+    assert (Fx.mx4_linear(x, w4).double() == 1.5 * scale).all()
+    dx = native().mx4_dgrad(dy, w4.codes, w4.scales).double()
+    assert (dx[:, 0] == 0.5 * scale).all() and (dx[:, 1] == scale).all() and (dx[:, 2:] == 0).all()

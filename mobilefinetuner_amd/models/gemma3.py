@@ -25,7 +25,7 @@ import torch.nn as nn
 from ..ops import functional as Fx
 from ..ops.rope_tables import rope_tables
 from ..parallel.sharder import gate
-from .layers import Linear, RMSNorm, mx4_weights, refuse_mx4
+from .layers import Linear, MX4Module, RMSNorm, mx4_weights, refuse_mx4
 
 
 def _pattern_layer_types(n_layers: int, pattern: int = 6):
@@ -159,7 +159,7 @@ class Gemma3Layer(nn.Module):
         return self.down_proj(Fx.gated_act(self.gate_up_proj(h), self.act, self.down_proj.aug_cols()))
 
 
-class Gemma3Model(nn.Module):
+class Gemma3Model(MX4Module):
     def __init__(self, cfg: Gemma3Config, dtype=torch.bfloat16, device="cuda", init: bool = True, seed: int = 0,
                  rope_len: int | None = None):
         super().__init__()

@@ -21,7 +21,7 @@ import torch.nn as nn
 
 from ..ops import functional as Fx
 from ..parallel.sharder import gate
-from .layers import LayerNorm, Linear, mx4_weights, refuse_mx4
+from .layers import LayerNorm, Linear, MX4Module, mx4_weights, refuse_mx4
 
 
 @dataclass
@@ -104,7 +104,7 @@ class GPT2Block(nn.Module):
         return Fx.mlp_gelu(h, self.c_fc, self.mlp_proj)
 
 
-class GPT2Model(nn.Module):
+class GPT2Model(MX4Module):
     """forward(input_ids[B,S], labels[B,S] shifted targets) -> mean loss; or final hidden."""
 
     def __init__(self, cfg: GPT2Config, dtype=torch.bfloat16, device="cuda", init: bool = True, seed: int = 0):

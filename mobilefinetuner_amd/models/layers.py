@@ -32,6 +32,40 @@ def refuse_mx4(model, what: str):
         raise RuntimeError(f"{what}: not on a 4-bit base (peft.mx4.quantize_base)")
 
 
+class MX4Module(nn.Module):
+    """A module whose weights may be MX4Weights: no parameters, but moved with the module (``model.to(device)``) and part of
+    its state dict as ``<name>_codes`` and ``<name>_scales``, which a model of the same quantised base loads."""
+
+    def _mx4(self):
+        return [(k, w) for k, w in self.__dict__.items() if isinstance(w, MX4Weight)]
+
+    def _apply(self, fn, recurse=True):
+        for k, w in self._mx4():
+            self.__dict__[k] = MX4Weight(fn(w.codes), fn(w.scales))
+        return super()._apply(fn, recurse)
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        for k, w in self._mx4():
+            destination[f"{prefix}{k}_codes"], destination[f"{prefix}{k}_scales"] = w.codes, w.scales
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        for k, w in self._mx4():
+            for part in ("codes", "scales"):
+                key, dst = f"{prefix}{k}_{part}", getattr(w, part)
+                src = state_dict.get(key)
+                if src is None:
+                    if strict:
+                        missing_keys.append(key)
+                elif src.shape != dst.shape or src.dtype != dst.dtype:
+                    error_msgs.append(f"{key}: {src.dtype} {tuple(src.shape)}, expected {dst.dtype} {tuple(dst.shape)}")
+                else:
+                    dst.copy_(src)
+                if key in unexpected_keys:
+                    unexpected_keys.remove(key)
+
+
 @dataclass
 class LoRASlice:
     """One LoRA adapter on columns [col0, col0 + ncols) of a (possibly fused) linear output.
@@ -44,7 +78,7 @@ class LoRASlice:
     name: str = ""
 
 
-class Linear(nn.Module):
+class Linear(MX4Module):
     def __init__(self, in_features, out_features, bias=True, dtype=torch.bfloat16, device=None):
         super().__init__()
         self.in_features, self.out_features = in_features, out_features

@@ -87,3 +87,34 @@ def test_clis(tmp_path):
                                 "--seq_len", "32", "--output_dir", str(tmp_path), "--targets", "full"])
     assert len(tr.history) == 2
     eval_ppl.main(["--model", "gpt2-tiny", *CPU, "--base_mx4", "--seq_len", "32", "--max_batches", "2", "--lora_path", out])
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "gemma"])
+def test_state_dict_holds_the_4_bit_base(kind):
+    from mobilefinetuner_amd.models.layers import mx4_weights
+    a, b = _model(kind), _model(kind)
+    for w in mx4_weights(b):
+        w.codes.fill_(0x11), w.scales.fill_(100)
+    sd = a.state_dict()
+    assert sum(k.endswith("_codes") for k in sd) == sum(k.endswith("_scales") for k in sd) == len(mx4_weights(a))
+    b.load_state_dict(sd)
+    for wa, wb in zip(mx4_weights(a), mx4_weights(b)):
+        assert torch.equal(wa.codes, wb.codes) and torch.equal(wa.scales, wb.scales)
+    name = ("wte" if kind == "gpt2" else "embed") + "_codes"
+    with pytest.raises(RuntimeError, match="Missing key"):
+        b.load_state_dict({k: v for k, v in sd.items() if k != name})
+    with pytest.raises(RuntimeError, match=f"{name}: "):
+        b.load_state_dict({**sd, name: sd[name][1:]})
+    with pytest.raises(RuntimeError, match="Unexpected key"):
+        _model(kind, quantize=False).load_state_dict(sd)
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "gemma"])
+def test_the_4_bit_base_moves_with_its_model(kind):
+    from mobilefinetuner_amd.models.layers import mx4_weights
+    m = _model(kind)
+    before = [(w.codes.clone(), w.scales.clone()) for w in mx4_weights(m)]
+    m.double()  # a change of type is the parameters' alone
+    assert all(torch.equal(w.codes, c) and torch.equal(w.scales, s) for w, (c, s) in zip(mx4_weights(m), before))
+    m.to("meta")
+    assert len(mx4_weights(m)) == len(before) and all(w.device.type == "meta" for w in mx4_weights(m))

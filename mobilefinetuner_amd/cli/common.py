@@ -100,6 +100,13 @@ def add_base_args(ap):
                         "adapters are trained and applied on top, never merged")
 
 
+def merge_adapter(a) -> bool:
+    """--lora_merge (the evaluation CLIs' default), except on a 4-bit base, which takes no adapter in."""
+    if a.lora_merge and a.base_mx4:
+        log0("  --lora_merge does not apply with --base_mx4: the adapter stays on top of the 4-bit base")
+    return bool(a.lora_merge) and not a.base_mx4
+
+
 def quantize_base(a, model):
     """--base_mx4, after the base weights are final."""
     if not a.base_mx4:

@@ -49,7 +49,7 @@ def main(argv=None):
     if a.lora_path:
         t, m = load_lora(a.lora_path)
         attach_lora(model, t, m)
-        if a.lora_merge and not a.base_mx4:
+        if common.merge_adapter(a):
             merge_all(model)
             set_lora_enabled(model, False)
         elif a.base_mx4 and dev.type == "cuda":  # a separate adapter: bf16 compute shadows of its fp32 A / B

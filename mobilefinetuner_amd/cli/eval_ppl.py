@@ -80,7 +80,7 @@ def main(argv=None):
         tensors, meta = load_lora(a.lora_path)
         spec = attach_lora(model, tensors, meta)
         log0(f"  ✓ LoRA attached: rank={spec.rank} alpha={spec.alpha:g}")
-        if a.lora_merge and not a.base_mx4:
+        if common.merge_adapter(a):
             merge_all(model)
             set_lora_enabled(model, False)
             log0("  ✓ LoRA merged into base weights")

@@ -118,3 +118,16 @@ def test_the_4_bit_base_moves_with_its_model(kind):
     assert all(torch.equal(w.codes, c) and torch.equal(w.scales, s) for w, (c, s) in zip(mx4_weights(m), before))
     m.to("meta")
     assert len(mx4_weights(m)) == len(before) and all(w.device.type == "meta" for w in mx4_weights(m))
+
+
+@pytest.mark.parametrize("cli", ["eval_ppl", "eval_mmlu"])
+def test_evaluation_says_that_a_4_bit_base_is_not_merged(cli, capsys):
+    import importlib
+    from mobilefinetuner_amd.cli import common
+    parser = importlib.import_module(f"mobilefinetuner_amd.cli.{cli}").build_parser()
+    need = ["--mmlu_root", "x"] if cli == "eval_mmlu" else []
+    assert not common.merge_adapter(parser.parse_args([*need, "--base_mx4"]))
+    assert "--lora_merge does not apply with --base_mx4" in capsys.readouterr().out
+    assert common.merge_adapter(parser.parse_args(need))
+    assert not common.merge_adapter(parser.parse_args([*need, "--base_mx4", "--lora_merge", "0"]))
+    assert capsys.readouterr().out == ""

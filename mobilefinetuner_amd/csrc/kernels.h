@@ -81,7 +81,8 @@ enum GemmEpi { GEMM_EPI_NONE = 0, GEMM_EPI_BIAS = 1, GEMM_EPI_BIAS_GELU = 2, GEM
                // [M, 2I] (ldc): dg = dh u gelu'(g), du = dh gelu(g)
                GEMM_EPI_GEGLU_FWD = 12, GEMM_EPI_GEGLU_BWD = 13,
                // CE_DGRAD of one piece of the vocabulary, added to a running fp32 sum (gemm8, NN, one split)
-               GEMM_EPI_CE_DGRAD_ACC = 14 };
+               GEMM_EPI_CE_DGRAD_ACC = 14,
+               GEMM_EPI_CE_DGRAD_ROWS = 15 };  // CE_DGRAD where b_rows < K (gemm8x picks it)
 struct GemmArgs {
   const bf16_t* A;
   long lda;  // A [M, K] row-major

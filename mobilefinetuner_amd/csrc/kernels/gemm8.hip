@@ -44,9 +44,10 @@ namespace {
 constexpr int kHalf = 128 * 64;  // elements in a half-tile
 
 typedef __attribute__((address_space(3))) void lds_void8;
-// the two LM-head CE data gradients: straight into dh (or split slabs), and into a running fp32 sum
+// the LM-head CE data gradients: straight into dh (or split slabs), the same over a table that ends early (b_rows), and into
+// a running fp32 sum
 template <int EPI>
-constexpr bool kCeDgrad = EPI == GEMM_EPI_CE_DGRAD || EPI == GEMM_EPI_CE_DGRAD_ACC;
+constexpr bool kCeDgrad = EPI == GEMM_EPI_CE_DGRAD || EPI == GEMM_EPI_CE_DGRAD_ROWS || EPI == GEMM_EPI_CE_DGRAD_ACC;
 
 typedef const __attribute__((address_space(1))) void g_void8;
 
@@ -127,7 +128,8 @@ __device__ __forceinline__ void stage_half_fast(bf16_t* lds, const bf16_t* src, 
 // bank slots -> conflict-free transposed reads.
 __device__ __forceinline__ int tsw(int k) { return ((k & 3) | (((k >> 3) & 1) << 2)) << 1; }
 
-// KC: rows past kmax - 1 read row kmax - 1
+// KC: rows past kmax - 1 read row kmax - 1.  (A minimum per load: the loss of 32768 x 262144 x 640 23.60 ms with it, 23.44
+// without, 65536 x 50304 x 768 9.50 and 9.49, so only the products over a table that ends early have it.)
 template <bool KC = false>
 __device__ __forceinline__ void stage_half_t(bf16_t* lds, const bf16_t* src, long ld, int c0, int cmax, int k0,
                                              int kmax = 0) {
@@ -754,7 +756,8 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
       if constexpr (AT) stage_half_t(half_ptr(buf, h), g.A, g.lda, m0 + h * 128, g.M, k0);
       else stage_half(half_ptr(buf, h), g.A, g.lda, m0 + h * 128, g.M, k0);
     } else {
-      if constexpr (kCeDgrad<EPI>) stage_half_t<true>(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0, g.b_rows ? g.b_rows : g.K);
+      if constexpr (EPI == GEMM_EPI_CE_DGRAD_ROWS || EPI == GEMM_EPI_CE_DGRAD_ACC)
+        stage_half_t<true>(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0, g.b_rows ? g.b_rows : g.K);
       else if constexpr (BT) stage_half_t(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0);
       else stage_half(half_ptr(buf, h), g.B, g.ldb, n0 + (h - 2) * 128, g.N, k0);
     }
@@ -1673,7 +1676,8 @@ void gemm8x(const GemmArgs& g0, int epi, bool a_t, bool b_t, hipStream_t st) {
                         "slab workspace and whole vocab tiles per split\n");
         abort();
       }
-      launch8<GEMM_EPI_CE_DGRAD, false, true>(g, st);
+      if (g.b_rows && g.b_rows < g.K) launch8<GEMM_EPI_CE_DGRAD_ROWS, false, true>(g, st);
+      else launch8<GEMM_EPI_CE_DGRAD, false, true>(g, st);
       break;
     case GEMM_EPI_CE_DGRAD_ACC:
       if (a_t || !b_t || g.ksplit > 1 || !g.ce_ratio || !g.ce_fin || !g.ce_acc) {

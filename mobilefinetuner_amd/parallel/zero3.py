@@ -448,6 +448,8 @@ def gemma_units(model):
 
 def attach_zero3(model, device, group=None, prefetch: bool = True, **adamw_kwargs) -> Zero3:
     """Partition a full-fine-tuning model's parameters (call after set_full_finetune())."""
+    from ..models.layers import refuse_mx4
+    refuse_mx4(model, "ZeRO-3")
     units = gemma_units(model) if hasattr(model, "layers") else gpt2_units(model)
     z3 = Zero3(units, device, group=group, prefetch=prefetch, **adamw_kwargs)
     model.zero3 = z3

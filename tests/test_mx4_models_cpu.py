@@ -131,3 +131,10 @@ def test_evaluation_says_that_a_4_bit_base_is_not_merged(cli, capsys):
     assert common.merge_adapter(parser.parse_args(need))
     assert not common.merge_adapter(parser.parse_args([*need, "--base_mx4", "--lora_merge", "0"]))
     assert capsys.readouterr().out == ""
+
+
+@pytest.mark.parametrize("kind", ["gpt2", "gemma"])
+def test_zero3_refuses_a_4_bit_base(kind):
+    from mobilefinetuner_amd.parallel.zero3 import attach_zero3
+    with pytest.raises(RuntimeError, match="ZeRO-3: not on a 4-bit base"):
+        attach_zero3(_model(kind), torch.device("cpu"))

@@ -459,7 +459,7 @@ __device__ __forceinline__ void ce_exp_piece(f32x2_t& s, float& xl, bool& hit, b
     hit = true;
   }
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {  // packed fp32: the scale-and-shift and the running sums two at a time
+  for (int e = 0; e < 8; e += 2) {  // the scale-and-shift and the running sums as pairs: two sums, of the even and the odd columns
     const f32x2_t t = __builtin_elementwise_fma(f32x2_t{v[e], v[e + 1]}, f32x2_t{1.4426950408889634f, 1.4426950408889634f},
                                                 f32x2_t{-mb, -mb});
     v[e] = fast_exp2(t.x), v[e + 1] = fast_exp2(t.y);

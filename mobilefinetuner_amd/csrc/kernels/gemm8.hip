@@ -842,8 +842,8 @@ __global__ __launch_bounds__(512, 1) void gemm8_kernel(GemmArgs g) {
   // K-tile, inside the MFMA cluster: 4 v_mul_f32 fit the 16-cycle issue gap of the MFMA before (the
   // same multiplies placed in the load segment cost ~15% of the kernel: VALU there competes with
   // the partner wave's prio-1 MFMA cluster).  Branch-free (factor 1 off the tile starts): a
-  // second MFMA code path for the tile starts spills.  Scalar asm multiplies: left to the
-  // compiler they become v_pk_mul_f32, which costs extra cycles beside MFMAs.
+  // second MFMA code path for the tile starts spills.  The multiplies are asm so that each stays a
+  // v_mul_f32 of its own right where it is written.
   auto mma_ce = [&](int q, const f32x4_t& r) {
     if constexpr (kCeDgrad<EPI>) {
       __builtin_amdgcn_s_setprio(1);

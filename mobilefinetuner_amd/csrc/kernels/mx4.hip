@@ -236,8 +236,9 @@ __global__ __launch_bounds__(64 * (S > 4 ? S : 4)) void mx4_rows_kernel(Mx4Linea
 // Streams the codes once: a wave owns 32 columns and walks K in steps of 256, a lane reading 32 B of its row (two
 // scale groups: columns 256 s + 64 (l >> 4) .. + 63), so a step takes whole 128-B lines.  x sits in LDS, read with
 // the same permutation; rows M .. 15 of the operand repeat row M - 1 and are never stored.  No barrier in the loop.
-// 4 x 262144 x 1152: 37.5 us (4.4 TB/s of codes; the same through the tiles of mx4_gemm 43 us, through mx4_rows 45 us).
-// Measured and not kept: waves that go on to further strips with x already in LDS (38.4 us), 8 waves per SIMD (spills).
+// 4 x 262144 x 1152: 35.7 us (4.5 TB/s of codes and scales; the same through the tiles of mx4_gemm 43 us, through mx4_rows
+// 45 us).  Measured and not kept: waves that go on to further strips with x already in LDS (0.9 us more), 8 waves per SIMD
+// (spills).
 __global__ __launch_bounds__(256) void mx4_stream_kernel(Mx4LinearArgs g) {
   extern __shared__ __attribute__((aligned(16))) bf16_t xs[];
   constexpr int TN = 2;

@@ -186,19 +186,11 @@ void Zero3::shard_optimizer(AdamW& opt, bool host_moments, bool host_fp32, bool 
   for (auto& e : upd_ev_) HIP_OK(hipEventCreateWithFlags(&e, hipEventDisableTiming));
   HIP_OK(hipEventCreateWithFlags(&fork_ev_, hipEventDisableTiming));
   HIP_OK(hipEventCreateWithFlags(&ojoin_ev_, hipEventDisableTiming));
-  // the updates run beside the forward's kernels: a low-priority stream and a bounded grid (the
-  // kernel waits on PCIe, not on the CU)
-  const char* pr = std::getenv("MFT_Z3_OPT_PRIO");
+  // the updates run beside the forward's kernels: a stream of their own and a bounded grid (the
+  // kernel waits on PCIe, not on the CU).  Default priority, as every stream here: kernels on streams of
+  // different priorities can wait for each other for good (two ranks with this stream at the lowest one did)
   const char* stg = std::getenv("MFT_Z3_STAGED");
-  if (!(stg && stg[0] == '0')) {
-    // (staged: no optimizer stream)
-  } else if (!(pr && pr[0] == '0')) {
-    int least = 0, greatest = 0;
-    HIP_OK(hipDeviceGetStreamPriorityRange(&least, &greatest));
-    HIP_OK(hipStreamCreateWithPriority(&ostream_, hipStreamNonBlocking, least));
-  } else {
-    HIP_OK(hipStreamCreateWithFlags(&ostream_, hipStreamNonBlocking));
-  }
+  if (stg && stg[0] == '0') HIP_OK(hipStreamCreateWithFlags(&ostream_, hipStreamNonBlocking));  // (staged: none)
   const char* gr = std::getenv("MFT_Z3_OPT_GRID");
   opt_grid_ = gr ? std::atoi(gr) : 32;  // profiles/r4_offload_modes.txt: 32 best of 16-2048
   const char* st = std::getenv("MFT_Z3_STAGED");

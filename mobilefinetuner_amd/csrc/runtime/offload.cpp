@@ -51,10 +51,8 @@ void HostTier::add(const std::string& name, size_t nbytes) {
     throw std::runtime_error("HostTier: entry " + name + " (" + std::to_string(nbytes) +
                              " B) exceeds the device budget (" + std::to_string(budget_) + " B)");
   if (!copy_) {
-    // high priority copy stream so prefetches are not starved by compute
-    int lo = 0, hi = 0;
-    HT_CHECK(hipDeviceGetStreamPriorityRange(&lo, &hi));
-    HT_CHECK(hipStreamCreateWithPriority(&copy_, hipStreamNonBlocking, hi));
+    // default priority, as every stream here: work on streams of different priorities can hang
+    HT_CHECK(hipStreamCreateWithFlags(&copy_, hipStreamNonBlocking));
     HT_CHECK(hipEventCreateWithFlags(&order_ev_, hipEventDisableTiming));
   }
   Entry e;

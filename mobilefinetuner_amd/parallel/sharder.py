@@ -9,8 +9,8 @@ called from the model forward per block (graph/gpt2_model.cpp:536-554).  The ref
 tensors stayed alive while the autograd graph referenced them ("real savings are bounded").
 
 MI355X design: the native HostTier (csrc/runtime/offload.cpp) holds the bytes in pinned DRAM (and
-optionally spills to ``--shard_dir`` files), copies run as hipMemcpyAsync on a high-priority copy
-stream ordered with hipEvents; eviction frees the DEVICE STORAGE in place (``storage.resize_(0)``),
+optionally spills to ``--shard_dir`` files), copies run as hipMemcpyAsync on a copy stream of their own
+ordered with hipEvents; eviction frees the DEVICE STORAGE in place (``storage.resize_(0)``),
 so tensors captured by autograd are released too and are re-filled in place before the backward of
 their block (a gate autograd node at each block boundary calls ``require`` on the way back).
 Frozen weights are bf16 already, so the host copy keeps the device dtype (the reference's

@@ -1,0 +1,21 @@
+"""Every HIP stream of the framework has the default priority (no GPU): work on streams of different priorities can hang."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _sources(*suffixes):
+    for base in ("mobilefinetuner_amd", "scripts", "tests"):
+        for folder, _, files in os.walk(os.path.join(ROOT, base)):
+            for f in files:
+                if f.endswith(suffixes) and f != os.path.basename(__file__):
+                    p = os.path.join(folder, f)
+                    with open(p, encoding="utf-8") as h:
+                        yield os.path.relpath(p, ROOT), h.read()
+
+
+def test_streams_have_the_default_priority():
+    bad = [p for p, s in _sources(".cpp", ".h", ".hip") if re.search(r"Stream(Create)?With(CUMask|Priority)\s*\(", s)]
+    bad += [p for p, s in _sources(".py") if re.search(r"Stream\([^)]*priority\s*=|is_high_priority_stream\s*=\s*True", s)]
+    assert not bad, bad

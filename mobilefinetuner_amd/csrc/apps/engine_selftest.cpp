@@ -120,6 +120,18 @@ int main() {
       return r;
     }(), 1e-2);
   }
+  // ---------------------------------------------------------------- zero_ at any address and length
+  for (DType dt : {DType::BF16, DType::F32}) {
+    bool ok = true;
+    for (int64_t lo : {0, 1, 3, 7, 8, 13})
+      for (int64_t n : {0, 1, 2, 7, 8, 9, 31, 4096, 70001}) {
+        Tensor t = full({lo + n + 19}, 1.0, dt);
+        t.slice(0, lo, lo + n).zero_();
+        const std::vector<double> v = host(t);
+        for (int64_t i = 0; i < (int64_t)v.size(); ++i) ok = ok && v[i] == (i >= lo && i < lo + n ? 0.0 : 1.0);
+      }
+    expect(dt == DType::F32 ? "zero_ of slices fp32" : "zero_ of slices bf16", ok);
+  }
   // ---------------------------------------------------------------- unary
   {
     auto x = rnd(1000, -3, 3);

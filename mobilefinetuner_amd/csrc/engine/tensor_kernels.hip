@@ -11,6 +11,7 @@
 
 #include "common.h"
 #include "engine/tensor_kernels.h"
+#include "kernels.h"
 
 namespace mft {
 namespace eng {
@@ -474,7 +475,7 @@ void fill(const Desc& d, double v, hipStream_t stm) {
   const int64_t n = numel(d);
   if (n == 0) return;
   if (v == 0.0 && contiguous(d)) {
-    MFT_HIP_CHECK(hipMemsetAsync(d.ptr, 0, (size_t)n * dsize(d.dtype), stm));
+    ::mft::zero_bytes(d.ptr, (size_t)n * dsize(d.dtype), stm);
     return;
   }
   fill_kernel<<<grid_for(n), 256, 0, stm>>>(d, v, n);

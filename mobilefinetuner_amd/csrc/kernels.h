@@ -427,6 +427,8 @@ void mx4_pad_rows(const bf16_t* in, long ldi, long rows, int width, bf16_t* out,
 void mx4_dense(const Mx4LinearArgs& a, bf16_t* w, bool dgrad, hipStream_t st);
 
 // ---------------------------------------------------------------- misc (misc.hip)
+// memory set to 0 by a kernel: a hipMemsetAsync node of a captured graph has given wrong results on replays after the first
+void zero_bytes(void* p, size_t bytes, hipStream_t st);
 void cast_f32_bf16(const float* x, bf16_t* y, long n, hipStream_t st);
 void cast_bf16_f32(const bf16_t* x, float* y, long n, hipStream_t st);
 void scale_bf16(const bf16_t* x, bf16_t* y, long n, const float* scale_dev, float scale, hipStream_t st);

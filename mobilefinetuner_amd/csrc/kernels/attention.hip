@@ -1830,7 +1830,7 @@ static void bwd_launch(const AttnBwdArgs& a, hipStream_t stream) {
     attn_bwd_delta_kernel<D><<<cdiv(rows * (D / 8), 256), 256, 0, stream>>>(a.o, a.dout, a.delta, mk(a.o_st),
                                                                             mk(a.do_st), a.B, a.H, a.Sq);
   }
-  MFT_HIP_CHECK(hipMemsetAsync(a.dq_acc, 0, sizeof(float) * (size_t)a.B * a.Sq * a.H * D, stream));
+  zero_bytes(a.dq_acc, sizeof(float) * (size_t)a.B * a.Sq * a.H * D, stream);
   const size_t shm = sizeof(bf16_t) * (2 * BK * D + 2 * BQ * D + 2 * BK * LDT) + sizeof(float) * 2 * BQ;
   static bool attr_set = false;
   if (!attr_set) {

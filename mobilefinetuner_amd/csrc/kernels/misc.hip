@@ -5,11 +5,30 @@
 #include "common.h"
 #include "kernels.h"
 
+#include <algorithm>
+
 namespace mft {
 
 static inline int grid_for(long n8) {
   long g = (n8 + 255) / 256;
   return (int)(g < 8192 ? (g > 0 ? g : 1) : 8192);
+}
+
+// head bytes up to a 16-byte boundary, n16 words of 16 bytes, tail bytes
+__global__ __launch_bounds__(256) void zero_bytes_kernel(char* __restrict__ p, int head, long n16, int tail) {
+  if (blockIdx.x == 0) {
+    if ((int)threadIdx.x < head) p[threadIdx.x] = 0;
+    if ((int)threadIdx.x < tail) p[head + n16 * 16 + threadIdx.x] = 0;
+  }
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n16; i += (long)gridDim.x * 256) q[i] = uint4{0, 0, 0, 0};
+}
+
+void zero_bytes(void* p, size_t bytes, hipStream_t st) {
+  if (!bytes) return;
+  const size_t head = std::min(bytes, (size_t)(-reinterpret_cast<uintptr_t>(p) & 15));
+  const long n16 = (long)((bytes - head) / 16);
+  zero_bytes_kernel<<<grid_for(n16), 256, 0, st>>>(static_cast<char*>(p), (int)head, n16, (int)(bytes - head - n16 * 16));
 }
 
 __global__ void cast_f32_bf16_kernel(const float* __restrict__ x, bf16_t* __restrict__ y, long n) {

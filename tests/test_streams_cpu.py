@@ -19,3 +19,11 @@ def test_streams_have_the_default_priority():
     bad = [p for p, s in _sources(".cpp", ".h", ".hip") if re.search(r"Stream(Create)?With(CUMask|Priority)\s*\(", s)]
     bad += [p for p, s in _sources(".py") if re.search(r"Stream\([^)]*priority\s*=|is_high_priority_stream\s*=\s*True", s)]
     assert not bad, bad
+
+
+def test_memory_is_cleared_by_kernels():
+    """hipMemsetAsync recorded into a graph has given wrong results on replays after the first.  gemm_s clears its counters with
+    it where nothing is captured: it asks first."""
+    bad = [p for p, s in _sources(".cpp", ".h", ".hip")
+           if p.startswith("mobilefinetuner_amd") and re.search(r"\bhipMemset\w*Async\s*\(|\bhipMemsetD", s) and not p.endswith("gemm_s.hip")]
+    assert not bad, bad

@@ -1,14 +1,8 @@
-// libmft engine: collective communication -- RCCL and host-loopback backends, bootstrap,
-// watchdog (see comm.h).
+// libmft engine: collective communication -- RCCL and host-loopback backends, watchdog (see comm.h;
+// bootstrap.cpp has the sockets between the ranks).
 #include "engine/comm.h"
 
-#include <arpa/inet.h>
-#include <netdb.h>
-#include <netinet/in.h>
-#include <netinet/tcp.h>
 #include <rccl/rccl.h>
-#include <sys/socket.h>
-#include <sys/time.h>
 #include <unistd.h>
 
 #include <algorithm>
@@ -27,6 +21,7 @@
 #include <thread>
 #include <vector>
 
+#include "engine/bootstrap.h"
 #include "engine/tensor.h"
 #include "engine/tensor_kernels.h"
 
@@ -36,105 +31,6 @@ namespace eng {
 size_t comm_type_size(CommType t) { return t == CommType::BF16 ? 2 : 4; }
 
 namespace {
-
-int env_int(const char* k, int dflt) {
-  const char* v = std::getenv(k);
-  return v && *v ? std::atoi(v) : dflt;
-}
-
-double comm_timeout_s() { return (double)env_int("MFT_COMM_TIMEOUT", 600); }
-
-bool send_all(int fd, const void* p, size_t n) {
-  const char* c = static_cast<const char*>(p);
-  while (n) {
-    const ssize_t k = ::send(fd, c, n, MSG_NOSIGNAL);
-    if (k <= 0) return false;
-    c += k;
-    n -= (size_t)k;
-  }
-  return true;
-}
-
-bool recv_all(int fd, void* p, size_t n) {
-  char* c = static_cast<char*>(p);
-  while (n) {
-    const ssize_t k = ::recv(fd, c, n, 0);
-    if (k <= 0) return false;
-    c += k;
-    n -= (size_t)k;
-  }
-  return true;
-}
-
-constexpr uint32_t kMagic = 0x4D465443;  // "MFTC": guards against a stray listener on the port
-
-int comm_port() { return env_int("MFT_COMM_PORT", env_int("MASTER_PORT", 29500) + 1); }
-
-sockaddr_in master_sockaddr() {
-  const char* a = std::getenv("MASTER_ADDR");
-  const std::string ip = resolve_ipv4(a && *a ? a : "127.0.0.1");
-  sockaddr_in sa{};
-  sa.sin_family = AF_INET;
-  sa.sin_port = htons((uint16_t)comm_port());
-  if (::inet_pton(AF_INET, ip.c_str(), &sa.sin_addr) != 1) throw std::runtime_error("comm: bad MASTER_ADDR " + ip);
-  return sa;
-}
-
-void tune_socket(int fd) {
-  int one = 1;
-  ::setsockopt(fd, IPPROTO_TCP, TCP_NODELAY, &one, sizeof(one));
-  timeval tv{};
-  tv.tv_sec = (long)comm_timeout_s();
-  ::setsockopt(fd, SOL_SOCKET, SO_RCVTIMEO, &tv, sizeof(tv));
-}
-
-// Star bootstrap: rank 0 listens and accepts world-1 connections (each peer sends magic + rank);
-// the others connect (retrying while rank 0 comes up).  Rank 0 gets fds[r] for r >= 1, every
-// other rank fds[0] = its connection to rank 0.
-std::vector<int> star_connect(int rank, int world) {
-  sockaddr_in sa = master_sockaddr();
-  std::vector<int> fds(world, -1);
-  if (rank == 0) {
-    const int lfd = ::socket(AF_INET, SOCK_STREAM, 0);
-    int one = 1;
-    ::setsockopt(lfd, SOL_SOCKET, SO_REUSEADDR, &one, sizeof(one));
-    if (::bind(lfd, reinterpret_cast<sockaddr*>(&sa), sizeof(sa)) != 0 || ::listen(lfd, world) != 0) {
-      ::close(lfd);
-      throw std::runtime_error("comm: rank 0 cannot listen on port " + std::to_string(comm_port()));
-    }
-    for (int i = 1; i < world; ++i) {
-      const int c = ::accept(lfd, nullptr, nullptr);
-      uint32_t hdr[2] = {0, 0};
-      if (c < 0 || !recv_all(c, hdr, sizeof(hdr)) || hdr[0] != kMagic || (int)hdr[1] <= 0 || (int)hdr[1] >= world ||
-          fds[hdr[1]] >= 0) {
-        ::close(lfd);
-        throw std::runtime_error("comm: bad bootstrap connection");
-      }
-      tune_socket(c);
-      fds[hdr[1]] = c;
-    }
-    ::close(lfd);
-    return fds;
-  }
-  const auto deadline = std::chrono::steady_clock::now() + std::chrono::duration<double>(comm_timeout_s());
-  while (true) {
-    const int fd = ::socket(AF_INET, SOCK_STREAM, 0);
-    if (::connect(fd, reinterpret_cast<const sockaddr*>(&sa), sizeof(sa)) == 0) {
-      const uint32_t hdr[2] = {kMagic, (uint32_t)rank};
-      if (!send_all(fd, hdr, sizeof(hdr))) {
-        ::close(fd);
-        throw std::runtime_error("comm: bootstrap send failed");
-      }
-      tune_socket(fd);
-      fds[0] = fd;
-      return fds;
-    }
-    ::close(fd);
-    if (std::chrono::steady_clock::now() > deadline)
-      throw std::runtime_error("comm: timed out connecting to rank 0 on port " + std::to_string(comm_port()));
-    std::this_thread::sleep_for(std::chrono::milliseconds(50));
-  }
-}
 
 // ---------------------------------------------------------------- host reductions (loopback)
 float bf16_to_f(uint16_t h) {
@@ -420,14 +316,14 @@ class LoopbackComm final : public Communicator {
   };
 
   void send_msg(int fd, const Op& o, const void* p, size_t bytes) {
-    const Hdr h{kMagic, o.kind, o.tag, 0, bytes};
+    const Hdr h{kCommMagic, o.kind, o.tag, 0, bytes};
     if (!send_all(fd, &h, sizeof(h)) || (bytes && !send_all(fd, p, bytes)))
       fail("loopback: a peer connection broke (send)");
   }
   void recv_msg(int fd, const Op& o, void* p, size_t bytes) {
     Hdr h{};
     if (!recv_all(fd, &h, sizeof(h))) fail("loopback: a peer disappeared or timed out (receive)");
-    if (h.magic != kMagic || h.kind != o.kind || h.tag != o.tag || h.bytes != bytes)
+    if (h.magic != kCommMagic || h.kind != o.kind || h.tag != o.tag || h.bytes != bytes)
       fail("loopback: collective mismatch between ranks (kind/tag/bytes " + std::to_string(h.kind) + "/" +
            std::to_string(h.tag) + "/" + std::to_string(h.bytes) + " vs " + std::to_string(o.kind) + "/" +
            std::to_string(o.tag) + "/" + std::to_string(bytes) + ")");
@@ -502,20 +398,6 @@ int64_t now_ns() {
 }
 
 }  // namespace
-
-std::string resolve_ipv4(const std::string& host) {
-  in_addr a{};
-  if (::inet_pton(AF_INET, host.c_str(), &a) == 1) return host;
-  addrinfo hints{}, *res = nullptr;
-  hints.ai_family = AF_INET;
-  hints.ai_socktype = SOCK_STREAM;
-  const int rc = ::getaddrinfo(host.c_str(), nullptr, &hints, &res);
-  if (rc != 0 || !res) throw std::runtime_error("comm: cannot resolve MASTER_ADDR '" + host + "': " + gai_strerror(rc));
-  char buf[INET_ADDRSTRLEN] = {0};
-  ::inet_ntop(AF_INET, &reinterpret_cast<sockaddr_in*>(res->ai_addr)->sin_addr, buf, sizeof(buf));
-  ::freeaddrinfo(res);
-  return buf;
-}
 
 // ---------------------------------------------------------------- watchdog
 struct Communicator::Watchdog {

@@ -110,8 +110,5 @@ class Communicator {
   std::unique_ptr<Watchdog> wd_;
 };
 
-// Resolve MASTER_ADDR (numeric IPv4 or a host name, getaddrinfo) to an IPv4 address string.
-std::string resolve_ipv4(const std::string& host);
-
 }  // namespace eng
 }  // namespace mft

@@ -187,8 +187,8 @@ void Zero3::shard_optimizer(AdamW& opt, bool host_moments, bool host_fp32, bool 
   HIP_OK(hipEventCreateWithFlags(&fork_ev_, hipEventDisableTiming));
   HIP_OK(hipEventCreateWithFlags(&ojoin_ev_, hipEventDisableTiming));
   // the updates run beside the forward's kernels: a stream of their own and a bounded grid (the
-  // kernel waits on PCIe, not on the CU).  Default priority, as every stream here: kernels on streams of
-  // different priorities can wait for each other for good (two ranks with this stream at the lowest one did)
+  // kernel waits on PCIe, not on the CU).  Default priority, as every stream here: work on streams of
+  // different priorities can hang
   const char* stg = std::getenv("MFT_Z3_STAGED");
   if (stg && stg[0] == '0') HIP_OK(hipStreamCreateWithFlags(&ostream_, hipStreamNonBlocking));  // (staged: none)
   const char* gr = std::getenv("MFT_Z3_OPT_GRID");

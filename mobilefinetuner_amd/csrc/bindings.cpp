@@ -973,6 +973,10 @@ PYBIND11_MODULE(_C, m) {
   m.def("mx4_linear", &mx4_linear);
   m.def("mx4_linear_grad", &mx4_linear_grad, "mx4_linear as an autograd node, gradient to x");
   m.def("mx4_dgrad", &mx4_dgrad);
+  m.def("mx4_plan", [](int M, int N, int K, bool dgrad) {
+    const auto p = mft::mx4_plan(M, N, K, dgrad, dgrad && N % 8 ? (N + 63) / 64 * 64 : (dgrad ? N : K));
+    return std::make_tuple(!dgrad && mft::mx4_few_rows(M, N, K) ? -mft::mx4_few_rows(M, N, K) : p.bm, p.tn, p.splits, p.dense);
+  }, "how a 4-bit product runs: (rows of a tile, its 64-column strips, splits, through a bf16 copy); rows -1 or -2: the kernels for few rows");
   m.def("lm_head_ce_pieces", &lm_head_ce_pieces);
   m.def("lm_head_ce_pieces_grad", &lm_head_ce_pieces_grad, "the loss as an autograd node, gradient to h");
   m.def("lm_head_ce_pieces_width", &mft::lm_head_ce_pieces_width, py::arg("M"), py::arg("V"), py::arg("piece") = 0,

@@ -499,3 +499,11 @@ def test_smallest_scales_in_products(m, n, byte):
     assert (Fx.mx4_linear(x, w4).double() == 1.5 * scale).all()
     dx = native().mx4_dgrad(dy, w4.codes, w4.scales).double()
     assert (dx[:, 0] == 0.5 * scale).all() and (dx[:, 1] == scale).all() and (dx[:, 2:] == 0).all()
+
+
+SPLIT_16 = [(31, 403, 3680), (17, 28, 9088)]  # tiles of 16 rows that share out their reduction
+
+
+@pytest.mark.parametrize("m,n,k", SPLIT_16)
+def test_small_tiles_that_split(m, n, k):
+    test_large_and_ragged_products(m, n, k)
